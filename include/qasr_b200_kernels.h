@@ -112,6 +112,117 @@ qasr_status qasr_kernel_kv_append(int device, void* stream, const uint16_t* k, c
                                   int layers, int nkv, int layer, const int* row_slot,
                                   const int* row_pos, int rows, char* err, int errlen);
 
+/* ------------------------------------------------------------------ serving over the paged cache
+ * A serving step on the device, with no read-back of lengths to the host: qasr_kernel_kv_plan
+ * gives each request the pages and row maps of its new positions, the projections may read 4-bit
+ * weights (qasr_kernel_gemv_w4), qasr_kernel_kv_append writes the new rows, and
+ * qasr_kernel_attention_chunk attends them.  No counterpart in the reference, whose decoder
+ * keeps one contiguous cache per slot (fork_capped, src/decoder.rs:2453).
+ * These calls allocate nothing and keep nothing between calls, so they may be captured into a
+ * CUDA graph, and they leave the calling thread's current device as it was. */
+
+/* Element types of activations and caches. */
+enum {
+  QASR_TYPE_F16 = 0,
+  QASR_TYPE_BF16 = 1
+};
+
+#define QASR_KV_PLAN_MAX_SEQS 8192
+#define QASR_KV_PLAN_MAX_SLOTS 65536
+
+/* Page table entries and row maps of one step, from the requests' lengths (device int32
+ * arrays).  Request i (0 <= i < n_seqs) holds kv_len[i] positions in slot seq_slot[i] and adds
+ * new_len[i] >= 0 (new_len NULL: one each).  With pages of 64 positions:
+ *   cu_rows[0] = 0, cu_rows[i+1] = cu_rows[i] + new_len[i]              (n_seqs + 1 entries)
+ *   row_slot[r] = seq_slot[i], row_pos[r] = kv_len[i] + r - cu_rows[i]  (cu_rows[i] <= r < cu_rows[i+1])
+ *   kv_len_out[i] = kv_len[i] + new_len[i]
+ *   the pages that request i lacks are popped off the free stack free_pages[0 .. *free_count),
+ *   the topmost first, in request order, into page_table[seq_slot[i]][...];
+ *   *free_count_out = *free_count - pages popped.
+ * row_slot / row_pos hold rows_cap entries; those behind the last row are left as they were.
+ * kv_len_out may be kv_len and free_count_out may be free_count (a step replayed in a graph then
+ * advances its own state); no other arrays may overlap.
+ * All or nothing: status (two int32 on the device) is {0, 0}, or {code, where} with
+ *   code QASR_ERR_INVALID_ARG: where = the first request whose slot is outside [0, max_slots) or
+ *     is listed before, whose kv_len is outside [0, max_pages * 64] or whose new_len is negative;
+ *     where = -3: *free_count outside [0, pool_pages];
+ *   code QASR_ERR_CAPACITY: where = the first request that does not fit max_pages * 64
+ *     positions; -1: the free stack is too short; -2: more rows than rows_cap.
+ * (Invalid arguments come before capacity, the requests before -1, -1 before -2.)
+ * Then every cu_rows entry is 0 (the step has no rows), kv_len_out = kv_len, free_count_out =
+ * free_count and nothing else is written.  The page ids on the stack are taken as given.
+ * n_seqs <= QASR_KV_PLAN_MAX_SEQS, max_slots <= QASR_KV_PLAN_MAX_SLOTS, max_pages < 2^25. */
+qasr_status qasr_kernel_kv_plan(int device, void* stream, const int* seq_slot, const int* kv_len,
+                                const int* new_len, int n_seqs, int max_slots, int* page_table,
+                                int max_pages, const int* free_pages, int pool_pages,
+                                const int* free_count, int* kv_len_out, int* free_count_out,
+                                int* cu_rows, int* row_slot, int* row_pos, int rows_cap, int* status,
+                                char* err, int errlen);
+
+/* Give the pages of finished requests back: free_pages[*free_count + ...] receives, in request
+ * order, the ceil(kv_len[i] / 64) pages of page_table[seq_slot[i]] in table order; kv_len_out[i] =
+ * 0, *free_count_out = *free_count + the pages pushed.  The table keeps its entries.  The same
+ * aliasing, limits and status as qasr_kernel_kv_plan; {QASR_ERR_CAPACITY, -1} when the stack
+ * would hold more than pool_pages entries. */
+qasr_status qasr_kernel_kv_release(int device, void* stream, const int* seq_slot, const int* kv_len,
+                                   int n_seqs, int max_slots, const int* page_table, int max_pages,
+                                   int* free_pages, int pool_pages, const int* free_count,
+                                   int* kv_len_out, int* free_count_out, int* status, char* err,
+                                   int errlen);
+
+/* GQA attention of chunks of new tokens over the paged cache.  Request i has the query rows
+ * cu_rows[i] .. cu_rows[i+1]-1 and kv_len[i] cached positions, its new ones among them (what
+ * qasr_kernel_kv_plan writes: cu_rows and kv_len_out); its j-th of n rows stands at position
+ * p = kv_len[i] - n + j and attends the positions 0..p of slot seq_slot[i]:
+ *   out[r, h] = sum_{t<=p} softmax_t(scale * q[r, h] . k_t) v_t,   kv head = h / (nq / nkv)
+ * A row at p < 0 sees nothing and is written as zeros; rows that no request owns are left as they
+ * were.  Chunks of any length go into one call: a decode step is n = 1 everywhere.
+ * type: QASR_TYPE_F16 or QASR_TYPE_BF16, of q, out and the cache.  q [rows, q_ld], out [rows,
+ * out_ld]: q_ld, out_ld >= nq * 128 and multiples of 8, both pointers and kv_pool on 16-byte
+ * boundaries; out may not overlap q.  nq a multiple of nkv, nq / nkv <= 16.  kv_pool
+ * [pool_pages][layers][2][nkv][64][128] in the layout of qasr_kernel_attention; at most 2^31 - 1
+ * rows of 128.  page_table [max_slots][max_pages], max_pages < 2^25.
+ * What lies behind a request's last position in its last page is never used, whatever it holds,
+ * and neither do values at later positions reach earlier rows.  Device arrays outside their
+ * ranges cannot lead out of the buffers: cu_rows is cut to [0, rows], kv_len to max_pages * 64, a
+ * slot outside [0, max_slots) counts as an empty cache and a page outside [0, pool_pages) as zeros.
+ * Scores, softmax sums and outputs are held in f32; probabilities are rounded to `type` for the
+ * product with V.  The keys are cut over the GPU as the whole call's lengths allow, so the last
+ * bits of a row depend on the other rows of the call; the same call gives the same bits.
+ * ws: qasr_kernel_attention_chunk_workspace(device) bytes on a 256-byte boundary, of any content;
+ * calls that may overlap on the GPU (streams, captured graphs) need one each. */
+int64_t qasr_kernel_attention_chunk_workspace(int device);
+qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, const void* q, int q_ld,
+                                        void* out, int out_ld, int rows, const void* kv_pool,
+                                        int pool_pages, const int* page_table, int max_slots,
+                                        int max_pages, int layers, int nq, int nkv, int layer,
+                                        const int* seq_slot, const int* cu_rows, const int* kv_len,
+                                        int n_seqs, float scale, void* ws, int64_t ws_bytes, char* err,
+                                        int errlen);
+
+#define QASR_W4_MAX_ROWS 64
+
+/* 4-bit weights with group scales: W[m, c] = scale[m, c / group] * (code[m, c] - zero), group 32, 64
+ * or 128 along k, zero = zero[m, c / group] (0..15) or 8 without zero points.
+ * qasr_kernel_pack_w4 lays the row-major codes (uint8 [n_out, k / 2], even c in the low four
+ * bits), scales (f16 [n_out, k / group]) and zero points (uint8 [n_out, k / group] or NULL) out once
+ * into `packed` (qasr_kernel_w4_packed_bytes bytes, 16-byte aligned), in the order in which the
+ * product streams them.  n_out >= 1 of any size, k a multiple of group.
+ * qasr_kernel_w4_packed_bytes returns -1 for sizes that are refused. */
+int64_t qasr_kernel_w4_packed_bytes(int n_out, int k, int group, int has_zero);
+qasr_status qasr_kernel_pack_w4(int device, void* stream, const uint8_t* codes, const uint16_t* scale,
+                                const uint8_t* zero, int n_out, int k, int group, void* packed,
+                                char* err, int errlen);
+
+/* out[r, m] = type(sum_c W[m, c] x[r, c])                          (accumulate == 0)
+ * out[r, m] = type(f32(out[r, m]) + sum_c W[m, c] x[r, c])         (accumulate != 0)
+ * for 1 <= rows <= QASR_W4_MAX_ROWS; x [rows, ldx], out [rows, ldo] of `type`, ldx >= k a multiple
+ * of 8, ldo >= n_out, x on a 16-byte boundary; out may overlap neither x nor packed.  Codes and zero
+ * points enter the product exactly, each group's sum and the sum over groups are f32. */
+qasr_status qasr_kernel_gemv_w4(int device, void* stream, int type, const void* packed, int has_zero,
+                                int n_out, int k, int group, const void* x, int ldx, int rows, void* out,
+                                int ldo, int accumulate, char* err, int errlen);
+
 /* Number of kernels this library launched since load (all contexts and probes). */
 uint64_t qasr_kernel_launch_count(void);
 

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -37,6 +38,8 @@ STOP_EOS, STOP_MAX_TOKENS = 0, 1
 ENDOFTEXT_TOKEN_ID, IM_END_TOKEN_ID = 151643, 151645
 WEIGHTS_F16 = 0
 WEIGHTS_INT8 = 1
+TYPE_F16, TYPE_BF16 = 0, 1
+KV_PLAN_MAX_SEQS, KV_PLAN_MAX_SLOTS, W4_MAX_ROWS = 8192, 65536, 64
 WEIGHTS_INT8_F32 = 2  # int8 + f32 per-row scales (the INT8 export's own `.weight_scale`)
 FLAG_KEEP_LOGITS = 1
 FLAG_NO_GRAPH = 2
@@ -58,6 +61,8 @@ EXPORTED_SYMBOLS = (
     "qasr_kernel_pack_weights", "qasr_kernel_gemm", "qasr_kernel_gemm_traced", "qasr_kernel_attention",
     "qasr_kernel_attention_noalloc", "qasr_kernel_attention_traced", "qasr_kernel_kv_append",
     "qasr_kernel_launch_count",
+    "qasr_kernel_kv_plan", "qasr_kernel_kv_release", "qasr_kernel_attention_chunk_workspace",
+    "qasr_kernel_attention_chunk", "qasr_kernel_w4_packed_bytes", "qasr_kernel_pack_w4", "qasr_kernel_gemv_w4",
     "qasr_synth_key", "qasr_synth_normal_f16", "qasr_synth_uniform_ids",
     "qasr_synth_quantize_rows", "qasr_f32_to_f16", "qasr_f16_to_f32", "qasr_f32_to_f16_array",
     "qasr_f16_to_f32_array",
@@ -267,6 +272,16 @@ def _load() -> ctypes.CDLL:
     lib.qasr_kernel_attention_noalloc.argtypes = [I, P, P, I, P, P, P, I, I, I, I, P, P, I, ctypes.c_char_p, I]
     lib.qasr_kernel_kv_append.argtypes = [I, P, P, P, P, P, I, I, I, I, P, P, I, ctypes.c_char_p, I]
     lib.qasr_kernel_launch_count.restype = ctypes.c_uint64
+    lib.qasr_kernel_kv_plan.argtypes = [I, P, P, P, P, I, I, P, I, P, I, P, P, P, P, P, P, I, P, ctypes.c_char_p, I]
+    lib.qasr_kernel_kv_release.argtypes = [I, P, P, P, I, I, P, I, P, I, P, P, P, P, ctypes.c_char_p, I]
+    lib.qasr_kernel_attention_chunk_workspace.argtypes = [I]
+    lib.qasr_kernel_attention_chunk_workspace.restype = ctypes.c_int64
+    lib.qasr_kernel_attention_chunk.argtypes = [I, P, I, P, I, P, I, I, P, I, P, I, I, I, I, I, I, P, P, P, I,
+                                                ctypes.c_float, P, ctypes.c_int64, ctypes.c_char_p, I]
+    lib.qasr_kernel_w4_packed_bytes.argtypes = [I, I, I, I]
+    lib.qasr_kernel_w4_packed_bytes.restype = ctypes.c_int64
+    lib.qasr_kernel_pack_w4.argtypes = [I, P, P, P, P, I, I, I, P, ctypes.c_char_p, I]
+    lib.qasr_kernel_gemv_w4.argtypes = [I, P, I, P, I, I, I, I, P, I, I, P, I, I, ctypes.c_char_p, I]
     lib.qasr_synth_key.argtypes = [ctypes.c_uint64, ctypes.c_uint64]
     lib.qasr_synth_key.restype = ctypes.c_uint64
     lib.qasr_synth_normal_f16.argtypes = [P, ctypes.c_size_t, ctypes.c_uint64, ctypes.c_uint64,
@@ -832,6 +847,96 @@ def kernel_kv_append(device: int, stream: int, k_ptr: int, v_ptr: int, pool_ptr:
         raise DecoderError(st, err.value.decode(errors="replace"))
 
 
+# The serving calls below run once per layer and step: pointers go to the library as plain integers,
+# and the message buffer is kept per thread instead of made anew for each call.
+_op_local = threading.local()
+
+
+def _op_buf():
+    buf = getattr(_op_local, "buf", None)
+    if buf is None:
+        buf = _op_local.buf = ctypes.create_string_buffer(512)
+    return buf
+
+
+def kernel_kv_plan(device: int, stream: int, seq_slot_ptr: int, kv_len_ptr: int, new_len_ptr: int | None, n_seqs: int,
+                   max_slots: int, page_table_ptr: int, max_pages: int, free_pages_ptr: int, pool_pages: int,
+                   free_count_ptr: int, kv_len_out_ptr: int, free_count_out_ptr: int, cu_rows_ptr: int,
+                   row_slot_ptr: int, row_pos_ptr: int, rows_cap: int, status_ptr: int):
+    """Pages, row maps and lengths of a step whose request i adds new_len[i] positions (None: one
+    each) to the kv_len[i] it holds.  Refusals that depend on the lengths arrive in the device status
+    words {code, where}; the step then has no rows and nothing else changes."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_kv_plan(device, stream, seq_slot_ptr, kv_len_ptr, new_len_ptr, n_seqs, max_slots, page_table_ptr,
+                                 max_pages, free_pages_ptr, pool_pages, free_count_ptr, kv_len_out_ptr,
+                                 free_count_out_ptr, cu_rows_ptr, row_slot_ptr, row_pos_ptr, rows_cap, status_ptr, buf,
+                                 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
+def kernel_kv_release(device: int, stream: int, seq_slot_ptr: int, kv_len_ptr: int, n_seqs: int, max_slots: int,
+                      page_table_ptr: int, max_pages: int, free_pages_ptr: int, pool_pages: int, free_count_ptr: int,
+                      kv_len_out_ptr: int, free_count_out_ptr: int, status_ptr: int):
+    """Push the pages of finished requests back onto the free stack and zero their lengths."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_kv_release(device, stream, seq_slot_ptr, kv_len_ptr, n_seqs, max_slots, page_table_ptr, max_pages,
+                                    free_pages_ptr, pool_pages, free_count_ptr, kv_len_out_ptr, free_count_out_ptr,
+                                    status_ptr, buf, 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
+def kernel_attention_chunk_workspace(device: int) -> int:
+    """Bytes of workspace kernel_attention_chunk wants on `device` (256-byte aligned, any content)."""
+    n = lib.qasr_kernel_attention_chunk_workspace(device)
+    if n < 0:
+        raise DecoderError(1, f"no device {device}")
+    return n
+
+
+def kernel_attention_chunk(device: int, stream: int, type: int, q_ptr: int, q_ld: int, out_ptr: int, out_ld: int,
+                           rows: int, pool_ptr: int, pool_pages: int, page_table_ptr: int, max_slots: int,
+                           max_pages: int, layers: int, nq: int, nkv: int, layer: int, seq_slot_ptr: int,
+                           cu_rows_ptr: int, kv_len_ptr: int, n_seqs: int, ws_ptr: int, ws_bytes: int,
+                           scale: float = 128.0 ** -0.5):
+    """Causal GQA attention of each request's new rows (cu_rows, kv_len as kernel_kv_plan leaves them)
+    over its paged cache; one row per request is the decode form."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_attention_chunk(device, stream, type, q_ptr, q_ld, out_ptr, out_ld, rows, pool_ptr, pool_pages,
+                                         page_table_ptr, max_slots, max_pages, layers, nq, nkv, layer, seq_slot_ptr,
+                                         cu_rows_ptr, kv_len_ptr, n_seqs, scale, ws_ptr, ws_bytes, buf, 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
+def kernel_w4_packed_bytes(n_out: int, k: int, group: int, has_zero: bool = False) -> int:
+    """Bytes of the packed form of an [n_out, k] 4-bit weight."""
+    n = lib.qasr_kernel_w4_packed_bytes(n_out, k, group, int(has_zero))
+    if n < 0:
+        raise DecoderError(1, f"no 4-bit layout for n_out {n_out}, k {k}, group {group}")
+    return n
+
+
+def kernel_pack_w4(device: int, stream: int, codes_ptr: int, scale_ptr: int, zero_ptr: int | None, n_out: int, k: int,
+                   group: int, packed_ptr: int):
+    """Row-major codes, scales and (optional) zero points -> the layout kernel_gemv_w4 streams."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_pack_w4(device, stream, codes_ptr, scale_ptr, zero_ptr, n_out, k, group, packed_ptr, buf, 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
+def kernel_gemv_w4(device: int, stream: int, type: int, packed_ptr: int, has_zero: bool, n_out: int, k: int, group: int,
+                   x_ptr: int, ldx: int, rows: int, out_ptr: int, ldo: int, accumulate: bool = False):
+    """out[r] (+)= W x[r] for at most W4_MAX_ROWS rows, W the packed 4-bit weight."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_gemv_w4(device, stream, type, packed_ptr, has_zero, n_out, k, group, x_ptr, ldx, rows, out_ptr,
+                                 ldo, accumulate, buf, 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
 def kv_page_swizzle(pool: np.ndarray) -> np.ndarray:
     """Convert KV pool pages [..., 64, 128] between the logical row layout and the
     swizzled one the kernels use (dim d of position p at column ((d // 8) ^ (p % 8)) * 8
@@ -854,6 +959,9 @@ def version() -> str:
 __all__ = [
     "TextDecoder", "DecoderError", "SyntheticModel", "MODEL_PRESETS", "text_config",
     "build_rope_tables", "dim_map", "kernel_pack_weights", "kernel_gemm", "kernel_attention_noalloc", "kernel_attention", "kernel_kv_append",
+    "kernel_kv_plan", "kernel_kv_release", "kernel_attention_chunk_workspace", "kernel_attention_chunk",
+    "kernel_w4_packed_bytes", "kernel_pack_w4", "kernel_gemv_w4", "TYPE_F16", "TYPE_BF16", "KV_PLAN_MAX_SEQS",
+    "KV_PLAN_MAX_SLOTS", "W4_MAX_ROWS",
     "launch_count", "version", "WEIGHTS_F16", "WEIGHTS_INT8", "WEIGHTS_INT8_F32", "EXPORTED_SYMBOLS", "lib",
     "Checkpoint", "read_model_config", "ModelConfig", "batch_decode_backend", "STOP_EOS", "STOP_MAX_TOKENS",
     "ENDOFTEXT_TOKEN_ID", "IM_END_TOKEN_ID", "Session", "common_rows", "suppress_runs", "CHUNK_MAX_NEW",

@@ -1,0 +1,209 @@
+// C entry points of the serving step over the paged cache (include/qasr_b200_kernels.h):
+// page and row maps, chunk attention, 4-bit products.  The calls check their scalar arguments,
+// enqueue on the caller's stream and return; nothing is allocated, kept or synchronised, and the
+// thread's current device is put back.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdio>
+#include <mutex>
+#include <string>
+
+#include "attention_chunk.cuh"
+#include "gemv_w4.cuh"
+#include "host_gemm.cuh"
+#include "kv_plan.cuh"
+#include "qasr_b200_kernels.h"
+
+using namespace qasr;
+
+namespace {
+
+constexpr int kMaxDevices = 16;
+
+qasr_status op_err(char* err, int errlen, qasr_status s, const char* m) noexcept {
+  if (err && errlen > 0) std::snprintf(err, errlen, "%s", m);
+  return s;
+}
+qasr_status op_cuda(char* err, int errlen, cudaError_t e, const char* what) noexcept {
+  if (err && errlen > 0) std::snprintf(err, errlen, "%s: %s", what, cudaGetErrorString(e));
+  return QASR_ERR_DEVICE;
+}
+
+// `device` current for the call's length.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) noexcept {
+    error = device < 0 || device >= kMaxDevices ? cudaErrorInvalidDevice : cudaGetDevice(&before_);
+    if (error == cudaSuccess && before_ != device) {
+      error = cudaSetDevice(device);
+      changed_ = error == cudaSuccess;
+    }
+  }
+  ~DeviceScope() {
+    if (changed_) cudaSetDevice(before_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  cudaError_t error = cudaSuccess;
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+};
+
+bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+// kv_plan_kernel may want more than the 48 KB of dynamic shared memory a kernel has by default.
+cudaError_t plan_attrs(int device) noexcept {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t result[kMaxDevices] = {};
+  try {
+    std::call_once(once[device], [device] {
+      const int most = static_cast<int>(plan_smem_bytes(QASR_KV_PLAN_MAX_SEQS, QASR_KV_PLAN_MAX_SLOTS));
+      cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kv_plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      result[device] = e;
+    });
+  } catch (...) {
+    return cudaErrorUnknown;
+  }
+  return result[device];
+}
+
+template <bool RELEASE>
+qasr_status launch_plan(int device, void* stream, const PlanArgs& a, char* err, int errlen) {
+  DeviceScope dev(device);
+  if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
+  cudaError_t e = plan_attrs(device);
+  if (e != cudaSuccess) return op_cuda(err, errlen, e, "kernel attributes");
+  // one CTA while it can write everything in a few rounds, else a whole cluster
+  const bool small = a.n_seqs <= 256 && (RELEASE || a.rows_cap <= 4 * PLAN_THREADS);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(small ? 1 : PLAN_MAX_CLUSTER);
+  cfg.blockDim = dim3(PLAN_THREADS);
+  cfg.dynamicSmemBytes = plan_smem_bytes(a.n_seqs, a.max_slots);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cfg.gridDim.x;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  e = cudaLaunchKernelEx(&cfg, kv_plan_kernel<RELEASE>, a);
+  return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "kv plan launch");
+}
+
+bool bad_plan_sizes(int n_seqs, int max_slots, int max_pages, int pool_pages) {
+  return n_seqs <= 0 || n_seqs > QASR_KV_PLAN_MAX_SEQS || max_slots <= 0 || max_slots > QASR_KV_PLAN_MAX_SLOTS ||
+         max_pages <= 0 || max_pages >= (1 << 25) || pool_pages < 0;
+}
+
+bool bad_w4_sizes(int n_out, int k, int group) {
+  return n_out <= 0 || k <= 0 || (group != 32 && group != 64 && group != 128) || k % group != 0 ||
+         n_out > (1 << 30) || k > (1 << 30);
+}
+
+}  // namespace
+
+extern "C" {
+
+qasr_status qasr_kernel_kv_plan(int device, void* stream, const int* seq_slot, const int* kv_len, const int* new_len,
+                                int n_seqs, int max_slots, int* page_table, int max_pages, const int* free_pages,
+                                int pool_pages, const int* free_count, int* kv_len_out, int* free_count_out,
+                                int* cu_rows, int* row_slot, int* row_pos, int rows_cap, int* status, char* err,
+                                int errlen) {
+  if (!seq_slot || !kv_len || !page_table || !free_pages || !free_count || !kv_len_out || !free_count_out || !cu_rows ||
+      !row_slot || !row_pos || !status || rows_cap < 0 || bad_plan_sizes(n_seqs, max_slots, max_pages, pool_pages))
+    return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad kv plan arguments");
+  PlanArgs a{seq_slot, kv_len, new_len, n_seqs, max_slots, page_table, max_pages, const_cast<int*>(free_pages),
+             pool_pages, free_count, kv_len_out, free_count_out, cu_rows, row_slot, row_pos, rows_cap, status};
+  return launch_plan<false>(device, stream, a, err, errlen);
+}
+
+qasr_status qasr_kernel_kv_release(int device, void* stream, const int* seq_slot, const int* kv_len, int n_seqs,
+                                   int max_slots, const int* page_table, int max_pages, int* free_pages, int pool_pages,
+                                   const int* free_count, int* kv_len_out, int* free_count_out, int* status, char* err,
+                                   int errlen) {
+  if (!seq_slot || !kv_len || !page_table || !free_pages || !free_count || !kv_len_out || !free_count_out || !status ||
+      bad_plan_sizes(n_seqs, max_slots, max_pages, pool_pages))
+    return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad kv release arguments");
+  PlanArgs a{seq_slot, kv_len, nullptr, n_seqs, max_slots, const_cast<int*>(page_table), max_pages, free_pages,
+             pool_pages, free_count, kv_len_out, free_count_out, nullptr, nullptr, nullptr, 0, status};
+  return launch_plan<true>(device, stream, a, err, errlen);
+}
+
+int64_t qasr_kernel_attention_chunk_workspace(int device) {
+  return device < 0 || device >= kMaxDevices ? -1 : 256;
+}
+
+qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, const void* q, int q_ld, void* out,
+                                        int out_ld, int rows, const void* kv_pool, int pool_pages,
+                                        const int* page_table, int max_slots, int max_pages, int layers, int nq,
+                                        int nkv, int layer, const int* seq_slot, const int* cu_rows, const int* kv_len,
+                                        int n_seqs, float scale, void* ws, int64_t ws_bytes, char* err, int errlen) {
+  if (!q || !out || !kv_pool || !page_table || !seq_slot || !cu_rows || !kv_len || !ws || rows <= 0 || n_seqs <= 0 ||
+      pool_pages <= 0 || max_slots <= 0 || max_pages <= 0 || max_pages >= (1 << 25) || layers <= 0 || layer < 0 ||
+      layer >= layers || nkv <= 0 || nq <= 0 || nq % nkv != 0 || nq / nkv > 16 || nq > (1 << 20) ||
+      q_ld < nq * CHUNK_DIM || out_ld < nq * CHUNK_DIM || q_ld % 8 || out_ld % 8 || misaligned(q, 16) ||
+      misaligned(out, 16) || misaligned(kv_pool, 16) || misaligned(ws, 256) || !std::isfinite(scale) ||
+      (type != QASR_TYPE_F16 && type != QASR_TYPE_BF16) ||
+      static_cast<__int128>(pool_pages) * layers * 2 * nkv * CHUNK_PAGE > 0x7fffffff)
+    return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad chunk attention arguments");
+  DeviceScope dev(device);
+  if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
+  if (ws_bytes < qasr_kernel_attention_chunk_workspace(device))
+    return op_err(err, errlen, QASR_ERR_CAPACITY, "chunk attention workspace too small");
+  ChunkArgs a{q, q_ld, out, out_ld, rows, kv_pool, pool_pages, page_table, max_slots, max_pages, layers, nq, nkv, layer,
+              seq_slot, cu_rows, kv_len, n_seqs, scale * 1.4426950408889634f};
+  const long long units = static_cast<long long>(rows) * nq;
+  if ((units + 7) / 8 > 0x7fffffff) return op_err(err, errlen, QASR_ERR_CAPACITY, "too many rows");
+  const dim3 grid(static_cast<unsigned>((units + 7) / 8));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = type == QASR_TYPE_BF16 ? launch_k(attention_chunk_rows_kernel<true>, grid, dim3(256), 0, st, true, a)
+                                               : launch_k(attention_chunk_rows_kernel<false>, grid, dim3(256), 0, st, true, a);
+  return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "chunk attention launch");
+}
+
+int64_t qasr_kernel_w4_packed_bytes(int n_out, int k, int group, int has_zero) {
+  return bad_w4_sizes(n_out, k, group) ? -1 : w4_layout(n_out, k, group, has_zero != 0).total;
+}
+
+qasr_status qasr_kernel_pack_w4(int device, void* stream, const uint8_t* codes, const uint16_t* scale,
+                                const uint8_t* zero, int n_out, int k, int group, void* packed, char* err, int errlen) {
+  if (!codes || !scale || !packed || bad_w4_sizes(n_out, k, group) || misaligned(packed, 16))
+    return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad w4 pack arguments");
+  DeviceScope dev(device);
+  if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
+  const cudaError_t e = launch_k(pack_w4_kernel, dim3(148 * 8), dim3(256), 0, static_cast<cudaStream_t>(stream), false,
+                                 codes, scale, zero, n_out, k, group, static_cast<uint8_t*>(packed));
+  return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "w4 pack launch");
+}
+
+qasr_status qasr_kernel_gemv_w4(int device, void* stream, int type, const void* packed, int has_zero, int n_out, int k,
+                                int group, const void* x, int ldx, int rows, void* out, int ldo, int accumulate,
+                                char* err, int errlen) {
+  if (!packed || !x || !out || bad_w4_sizes(n_out, k, group) || rows <= 0 || rows > QASR_W4_MAX_ROWS || ldx < k ||
+      ldx % 8 || ldo < n_out || misaligned(packed, 16) || misaligned(x, 16) || misaligned(out, 2) ||
+      (type != QASR_TYPE_F16 && type != QASR_TYPE_BF16))
+    return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad w4 gemv arguments");
+  DeviceScope dev(device);
+  if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
+  const W4Args a{static_cast<const uint8_t*>(packed), n_out, k, group == 32 ? 5 : group == 64 ? 6 : 7, x, ldx, rows, out,
+                 ldo, accumulate != 0};
+  const dim3 grid((n_out + 15) / 16);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool bf = type == QASR_TYPE_BF16;
+  const cudaError_t e = bf ? (has_zero ? launch_k(gemv_w4_kernel<true, true>, grid, dim3(W4_THREADS), 0, st, true, a)
+                                       : launch_k(gemv_w4_kernel<true, false>, grid, dim3(W4_THREADS), 0, st, true, a))
+                           : (has_zero ? launch_k(gemv_w4_kernel<false, true>, grid, dim3(W4_THREADS), 0, st, true, a)
+                                       : launch_k(gemv_w4_kernel<false, false>, grid, dim3(W4_THREADS), 0, st, true, a));
+  return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "w4 gemv launch");
+}
+
+}  // extern "C"
