@@ -62,7 +62,7 @@ EXPORTED_SYMBOLS = (
     "qasr_kernel_attention_noalloc", "qasr_kernel_attention_traced", "qasr_kernel_kv_append",
     "qasr_kernel_launch_count",
     "qasr_kernel_kv_plan", "qasr_kernel_kv_release", "qasr_kernel_attention_chunk_workspace",
-    "qasr_kernel_attention_chunk", "qasr_kernel_w4_packed_bytes", "qasr_kernel_pack_w4", "qasr_kernel_gemv_w4",
+    "qasr_kernel_attention_chunk", "qasr_kernel_attention_chunk_check", "qasr_kernel_w4_packed_bytes", "qasr_kernel_pack_w4", "qasr_kernel_gemv_w4",
     "qasr_synth_key", "qasr_synth_normal_f16", "qasr_synth_uniform_ids",
     "qasr_synth_quantize_rows", "qasr_f32_to_f16", "qasr_f16_to_f32", "qasr_f32_to_f16_array",
     "qasr_f16_to_f32_array",
@@ -278,6 +278,7 @@ def _load() -> ctypes.CDLL:
     lib.qasr_kernel_attention_chunk_workspace.restype = ctypes.c_int64
     lib.qasr_kernel_attention_chunk.argtypes = [I, P, I, P, I, P, I, I, P, I, P, I, I, I, I, I, I, P, P, P, I,
                                                 ctypes.c_float, P, ctypes.c_int64, ctypes.c_char_p, I]
+    lib.qasr_kernel_attention_chunk_check.argtypes = [I, P, P, ctypes.c_char_p, I]
     lib.qasr_kernel_w4_packed_bytes.argtypes = [I, I, I, I]
     lib.qasr_kernel_w4_packed_bytes.restype = ctypes.c_int64
     lib.qasr_kernel_pack_w4.argtypes = [I, P, P, P, P, I, I, I, P, ctypes.c_char_p, I]
@@ -910,6 +911,14 @@ def kernel_attention_chunk(device: int, stream: int, type: int, q_ptr: int, q_ld
         raise DecoderError(st, buf.value.decode(errors="replace"))
 
 
+def kernel_attention_chunk_check(device: int, stream: int, ws_ptr: int):
+    """Wait for the stream; raise if a device-side wait of the last kernel_attention_chunk over ws gave up."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_attention_chunk_check(device, stream, ws_ptr, buf, 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
 def kernel_w4_packed_bytes(n_out: int, k: int, group: int, has_zero: bool = False) -> int:
     """Bytes of the packed form of an [n_out, k] 4-bit weight."""
     n = lib.qasr_kernel_w4_packed_bytes(n_out, k, group, int(has_zero))
@@ -960,7 +969,7 @@ __all__ = [
     "TextDecoder", "DecoderError", "SyntheticModel", "MODEL_PRESETS", "text_config",
     "build_rope_tables", "dim_map", "kernel_pack_weights", "kernel_gemm", "kernel_attention_noalloc", "kernel_attention", "kernel_kv_append",
     "kernel_kv_plan", "kernel_kv_release", "kernel_attention_chunk_workspace", "kernel_attention_chunk",
-    "kernel_w4_packed_bytes", "kernel_pack_w4", "kernel_gemv_w4", "TYPE_F16", "TYPE_BF16", "KV_PLAN_MAX_SEQS",
+    "kernel_attention_chunk_check", "kernel_w4_packed_bytes", "kernel_pack_w4", "kernel_gemv_w4", "TYPE_F16", "TYPE_BF16", "KV_PLAN_MAX_SEQS",
     "KV_PLAN_MAX_SLOTS", "W4_MAX_ROWS",
     "launch_count", "version", "WEIGHTS_F16", "WEIGHTS_INT8", "WEIGHTS_INT8_F32", "EXPORTED_SYMBOLS", "lib",
     "Checkpoint", "read_model_config", "ModelConfig", "batch_decode_backend", "STOP_EOS", "STOP_MAX_TOKENS",

@@ -4,6 +4,33 @@
 // p = kv_len[i] - n_i + j) attends the positions 0..p of its slot:
 //   s_t = scale * q . k_t,   o = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m)
 // with the running maximum m and sum of an online softmax, so K and V are passed over once.
+//
+// The products are tcgen05 MMAs of 128 rows.  A kv head's nq / nkv = G query heads share its keys, so
+// the rows of a tile are packed: row r is token r / G, head r % G of the group (T tokens a tile, T the
+// largest multiple of 8 with T * G <= 128).  A block is two row tiles; per tile of 128 keys
+//   S = Q K^T        A: Q in shared memory, B: K in shared memory (positions x dims, K-major)
+//   P = 2^(S - m)    one thread per row, straight from and back to tensor memory, where P takes S's place
+//   O += P V         A: P in tensor memory, B: V in shared memory (MN-major), O in tensor memory
+// A page's swizzle (chunk c of position p at c ^ (p % 8)) is, for each 64-dim half of its rows, the
+// tensor core's own 128-byte swizzle, so pages are copied by TMA as they are and used as operands.
+// P is rounded to the cache's type for the second product, as the tensor core wants it; the sum of P
+// is taken before that rounding.  m is raised, and O rescaled, only when a row's maximum has grown by more than
+// 2^8 (P then stays below 2^8, far inside f16), so the rescaling, a round trip over O, is rare.
+//
+// Roles: warps 0-3 and 4-7 are two softmax groups, one per row tile; warps 8 and 9 issue the MMAs of one
+// group each; warp 10 copies Q and the pages into a ring of 128-position stages.  A block of one row tile only
+// (a decode step, a short chunk) gives its even key tiles to the first group and the odd ones to the second,
+// which then merge, so both always have work.
+//
+// Work split: every (request, kv head, block) costs its key tiles plus CHUNK_BLOCK_COST; the costs of the whole call,
+// laid end to end, are cut into one equal range per CTA.  A block that a cut goes through leaves f32
+// partials (o, m, l) in the workspace and attention_chunk_combine_kernel joins them, in key order.
+// Nothing about the lengths is known on the host: every CTA sums the costs itself.
+//
+// Masked keys: S is replaced, never added to, so whatever stands there cannot matter; their P is 0, and
+// V rows behind the block's last position are zeroed in shared memory, so that 0 * NaN cannot arise.  What remains
+// is a V that is not finite at a position which later rows of the same block may see and earlier ones may not: a row
+// whose result is not finite is computed again without matrix instructions (chunk_row).
 #pragma once
 #include <cuda_bf16.h>
 #include "device_common.cuh"
@@ -28,8 +55,38 @@ struct ChunkArgs {
   const int* cu_rows;
   const int* kv_len;
   int n_seqs;
-  float scale_log2;  // scale * log2(e): the softmax runs in powers of two
+  float scale_log2;  // |scale| * log2(e): the softmax runs in powers of two
+  int negate;        // the scale is negative
+  uint8_t* ws;       // ChunkMeta[grid], then the partials
 };
+
+constexpr int CHUNK_THREADS = 384;
+constexpr int CHUNK_KT = 128;                     // keys per tile
+constexpr int CHUNK_STAGES = 5;
+constexpr int CHUNK_STAGE_BYTES = CHUNK_KT * CHUNK_DIM * 2;
+constexpr int CHUNK_HALF_BYTES = CHUNK_KT * 128;  // 128 rows of one 64-dim half
+constexpr int CHUNK_Q_BYTES = 2 * CHUNK_STAGE_BYTES;
+constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + CHUNK_STAGES * CHUNK_STAGE_BYTES + 1536;
+constexpr int CHUNK_BLOCK_COST = 1;               // a block's Q copy, first and last steps, in key tiles
+constexpr int CHUNK_SNAP = 1;                     // a cut this near to a block's edge moves onto it
+constexpr float CHUNK_RESCALE = 8.0f;
+constexpr uint64_t CHUNK_WAIT_NS = 10 * QASR_WAIT_NS;  // rows computed again by chunk_row keep the others waiting
+constexpr int CHUNK_PART_ROWS = 256;
+constexpr int CHUNK_PART_FLOATS = (CHUNK_DIM + 2) * CHUNK_PART_ROWS;  // [o 0..127, m, l][row]
+
+struct ChunkMeta {
+  int state;  // 1: this CTA began a block that others finish; 2: a wait gave up
+  int row0, ntok, head, nt, pos0;
+  long long base, total;
+};
+__host__ __device__ constexpr long long chunk_meta_bytes(int grid) { return (grid * 64ll + 255) / 256 * 256; }
+__host__ __device__ constexpr long long chunk_ws_bytes(int grid) {
+  return chunk_meta_bytes(grid) + 2ll * grid * CHUNK_PART_FLOATS * 4;
+}
+__device__ __forceinline__ float* chunk_part(const ChunkArgs& a, int grid, int slot) {
+  return reinterpret_cast<float*>(a.ws + chunk_meta_bytes(grid)) + static_cast<size_t>(slot) * CHUNK_PART_FLOATS;
+}
+__host__ __device__ constexpr int chunk_tile_tokens(int group) { return (128 / group) & ~7; }
 
 template <bool BF16>
 struct ChunkType;
@@ -61,35 +118,160 @@ __device__ __forceinline__ long long chunk_kv_row(const ChunkArgs& a, int slot, 
   return (((static_cast<long long>(page) * a.layers + a.layer) * 2 + kv) * a.nkv + head) * CHUNK_PAGE + (t & 63);
 }
 
-// One warp per (row, query head): lane l holds dims 4l .. 4l + 3.
+// ---------------------------------------------------------------- the schedule
+struct ChunkSeq {
+  int row0, n, len, slot;  // first row, rows, cached positions (its rows' included), slot (-1: none)
+};
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkArgs& a, int i) {
+  ChunkSeq s;
+  s.row0 = min(max(a.cu_rows[i], 0), a.rows);
+  s.n = min(max(a.cu_rows[i + 1], 0), a.rows) - s.row0;
+  if (s.n < 0) s.n = 0;
+  s.slot = a.seq_slot[i];
+  if (s.slot < 0 || s.slot >= a.max_slots) s.slot = -1;
+  s.len = s.slot < 0 ? 0 : min(max(a.kv_len[i], 0), a.max_pages * CHUNK_PAGE);
+  return s;
+}
+// key tiles of block k (rows [k * bt, min(n, (k + 1) * bt)) of the request): at least one, so that a
+// block which sees nothing is visited and written
+__device__ __forceinline__ int chunk_tiles(const ChunkSeq& s, int k, int bt) {
+  const int end = s.len - s.n + min(s.n, (k + 1) * bt);
+  return max(1, (end + CHUNK_KT - 1) / CHUNK_KT);
+}
+__device__ __forceinline__ long long chunk_head_cost(const ChunkSeq& s, int bt) {
+  long long c = 0;
+  const int nb = (s.n + bt - 1) / bt;
+  for (int k = 0; k < nb; ++k) c += chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST;
+  return c;
+}
+__device__ __forceinline__ long long chunk_bound(long long total, int c, int grid) { return total * c / grid; }
+// The first key tile behind cut x of a block that starts at `base`.
+__device__ __forceinline__ int chunk_cut(long long x, long long base, int nt) {
+  const long long t = x - base - CHUNK_BLOCK_COST;
+  if (t >= nt) return nt;
+  if (t <= CHUNK_SNAP) return 0;
+  return nt - t <= CHUNK_SNAP ? nt : static_cast<int>(t);
+}
+
+struct ChunkWalk {
+  int i, g, k, nb, nt, t0, t1;
+  long long base, lo, hi;
+  ChunkSeq s;
+};
+// Fit the walk's block to the CTA's range; false past its end.  Blocks without a tile in the range are passed over.
+__device__ __forceinline__ bool chunk_fit(const ChunkArgs& a, ChunkWalk& w, int bt) {
+  while (w.i < a.n_seqs && w.base < w.hi) {
+    w.nt = chunk_tiles(w.s, w.k, bt);
+    w.t0 = chunk_cut(w.lo, w.base, w.nt);
+    w.t1 = chunk_cut(w.hi, w.base, w.nt);
+    if (w.t1 > w.t0) return true;
+    w.base += w.nt + CHUNK_BLOCK_COST;
+    if (++w.k == w.nb) {
+      w.k = 0;
+      if (++w.g == a.nkv) {
+        w.g = 0;
+        do {
+          if (++w.i >= a.n_seqs) return false;
+          w.s = chunk_seq(a, w.i);
+        } while (w.s.n == 0);
+        w.nb = (w.s.n + bt - 1) / bt;
+      }
+    }
+  }
+  return false;
+}
+__device__ __forceinline__ bool chunk_next(const ChunkArgs& a, ChunkWalk& w, int bt) {
+  w.base += w.nt + CHUNK_BLOCK_COST;
+  if (++w.k == w.nb) {
+    w.k = 0;
+    if (++w.g == a.nkv) {
+      w.g = 0;
+      do {
+        if (++w.i >= a.n_seqs) return false;
+        w.s = chunk_seq(a, w.i);
+      } while (w.s.n == 0);
+      w.nb = (w.s.n + bt - 1) / bt;
+    }
+  }
+  return chunk_fit(a, w, bt);
+}
+
+// ---------------------------------------------------------------- pieces
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y,
+                                            int32_t z, int32_t u) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(u)
+      : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Shared-memory descriptor of V as the second operand, MN-major with 128-byte swizzle: 64-dim halves
+// CHUNK_HALF_BYTES apart (LBO), groups of 8 positions 1024 bytes apart (SBO).
+__device__ __forceinline__ uint64_t smem_desc_v(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3fffu) | (static_cast<uint64_t>(CHUNK_HALF_BYTES >> 4) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) |
+         (static_cast<uint64_t>(2u) << 61);
+}
 template <bool BF16>
-__global__ void __launch_bounds__(256) attention_chunk_rows_kernel(const __grid_constant__ ChunkArgs a) {
+__host__ __device__ constexpr uint32_t chunk_idesc(bool b_mn_major) {
+  return umma_idesc_f16_m128(128) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u);
+}
+
+// A bounded wait of a whole warp: every lane sees the phase complete, or all of them give up together.
+__device__ __forceinline__ bool chunk_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = globaltimer();
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    int quit = 0;
+    if ((threadIdx.x & 31) == 0) {
+      if (*abort_flag) {
+        quit = 1;
+      } else if (globaltimer() - t0 > CHUNK_WAIT_NS) {
+        *abort_flag = 1;
+        quit = 1;
+      }
+    }
+    if (__shfl_sync(0xffffffffu, quit, 0)) return false;
+  }
+}
+
+// One row's (m, l, o) over the positions [t0, t1) without matrix instructions: a warp, lane l holding the dims
+// 4l .. 4l + 3.  For the rows whose tensor core result is not finite.
+template <bool BF16>
+__device__ __noinline__ void chunk_row(const ChunkArgs& a, const ChunkSeq& s, int row, int qhead, int t0, int t1,
+                                       float& m, float& l, float4& o) {
   using TT = ChunkType<BF16>;
   using T = typename TT::T;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const long long unit = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int r = static_cast<int>(unit / a.nq), h = static_cast<int>(unit % a.nq);
-  if (r >= a.rows) return;
-  int lo = 0, hi = a.n_seqs - 1;  // last request that starts at or before r
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu_rows[mid] <= r) lo = mid; else hi = mid - 1;
-  }
-  const int first = a.cu_rows[lo], end = min(a.cu_rows[lo + 1], a.rows);
-  if (r < first || r >= end) return;
-  const int slot = a.seq_slot[lo];
-  int len = slot >= 0 && slot < a.max_slots ? a.kv_len[lo] : 0;
-  len = static_cast<int>(min(static_cast<long long>(max(len, 0)), static_cast<long long>(a.max_pages) * 64));
-  const int last = len - (end - r);
-  const int head = h / (a.nq / a.nkv);
-  const T* qp = static_cast<const T*>(a.q) + static_cast<size_t>(r) * a.q_ld + h * CHUNK_DIM + lane * 4;
-  const uint2 qv = *reinterpret_cast<const uint2*>(qp);
+  const int lane = threadIdx.x & 31, head = qhead / (a.nq / a.nkv);
+  const uint2 qv = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) + static_cast<size_t>(row) * a.q_ld +
+                                                   qhead * CHUNK_DIM + lane * 4);
   const float2 q01 = TT::to_f32(qv.x), q23 = TT::to_f32(qv.y);
-  float m = -INFINITY, l = 0.0f, o[4] = {};
-  for (int t = 0; t <= last; ++t) {
-    const long long kr = chunk_kv_row(a, slot, t, 0, head), vr = chunk_kv_row(a, slot, t, 1, head);
+  m = -INFINITY;
+  l = 0.0f;
+  o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int t = t0; t < t1; ++t) {
+    const long long kr = chunk_kv_row(a, s.slot, t, 0, head), vr = chunk_kv_row(a, s.slot, t, 1, head);
     const int at = (((lane >> 1) ^ (t & 7)) << 3) + (lane & 1) * 4;
     uint2 kv = {}, vv = {};
     if (kr >= 0) {
@@ -97,26 +279,598 @@ __global__ void __launch_bounds__(256) attention_chunk_rows_kernel(const __grid_
       vv = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.pool) + vr * CHUNK_DIM + at);
     }
     const float2 k01 = TT::to_f32(kv.x), k23 = TT::to_f32(kv.y);
-    float s = q01.x * k01.x + q01.y * k01.y + q23.x * k23.x + q23.y * k23.y;
+    float d = q01.x * k01.x + q01.y * k01.y + q23.x * k23.x + q23.y * k23.y;
 #pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= a.scale_log2;
-    const float m2 = fmaxf(m, s);
+    for (int x = 16; x; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+    d *= a.negate ? -a.scale_log2 : a.scale_log2;
+    const float m2 = fmaxf(m, d);
     const float base = m2 == -INFINITY ? 0.0f : m2;
-    const float f = exp2f(m - base), p = exp2f(s - base);
+    const float f = ex2(m - base), p = ex2(d - base);
     const float2 v01 = TT::to_f32(vv.x), v23 = TT::to_f32(vv.y);
     l = l * f + p;
-    o[0] = o[0] * f + p * v01.x;
-    o[1] = o[1] * f + p * v01.y;
-    o[2] = o[2] * f + p * v23.x;
-    o[3] = o[3] * f + p * v23.y;
+    o.x = o.x * f + p * v01.x;
+    o.y = o.y * f + p * v01.y;
+    o.z = o.z * f + p * v23.x;
+    o.w = o.w * f + p * v23.y;
     m = m2;
   }
-  const float inv = last < 0 ? 0.0f : 1.0f / l;
-  uint2 res;
-  res.x = TT::from_f32(o[0] * inv, o[1] * inv);
-  res.y = TT::from_f32(o[2] * inv, o[3] * inv);
-  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(r) * a.out_ld + h * CHUNK_DIM + lane * 4) = res;
+  if (l != l) m = l;  // a score that is not a number: what joins this with other ranges must see it
+}
+
+struct ChunkBars {
+  uint64_t q_full, q_free, q_done;  // q_done: the block's last Q K^T of both groups is over
+  uint64_t kv_full[CHUNK_STAGES], kv_free[CHUNK_STAGES];
+  uint64_t s_full[2], p_full[2], pv_done[2], o_free[2], merge_full;
+  uint32_t tmem;
+  int abort_flag;
+  // the range's first block
+  int i, g, k, any;
+  long long base, total;
+  long long scan[CHUNK_THREADS / 32];
+};
+static_assert(sizeof(ChunkBars) <= 512, "ChunkBars sits in the last 512 bytes of the shared memory");
+
+// ring position of key tile j's K and V in a block of n tiles: K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1)
+__device__ __forceinline__ int chunk_k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int chunk_v_at(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
+
+template <bool BF16>
+__global__ void __launch_bounds__(CHUNK_THREADS, 1)
+    attention_chunk_kernel(const __grid_constant__ CUtensorMap q_big, const __grid_constant__ CUtensorMap q_small,
+                           const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ ChunkArgs a) {
+  using TT = ChunkType<BF16>;
+  using T = typename TT::T;
+  extern __shared__ __align__(1024) uint8_t chunk_dsmem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(chunk_dsmem) + 1023) & ~uintptr_t(1023));
+  uint8_t* sm_q = smem;                                    // two row tiles, each [2 halves][128 rows][128 B]
+  uint8_t* sm_kv = smem + CHUNK_Q_BYTES;                   // stages of [2 halves][128 positions][128 B]
+  float* sm_ml = reinterpret_cast<float*>(sm_kv + CHUNK_STAGES * CHUNK_STAGE_BYTES);  // [2][128]: group 1's m and l
+  ChunkBars& B = *reinterpret_cast<ChunkBars*>(reinterpret_cast<uint8_t*>(sm_ml) + 1024);
+  float* sm_o = reinterpret_cast<float*>(sm_q);            // [128 dims][128 rows]: group 1's O of a one-tile block
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int grid = gridDim.x, cta = blockIdx.x;
+  const int group = a.nq / a.nkv, T_tok = chunk_tile_tokens(group), bt = 2 * T_tok;
+
+  if (tid == 0) {
+    mbar_init(&B.q_full, 1);
+    mbar_init(&B.q_free, 6);
+    mbar_init(&B.q_done, 2);
+    for (int i = 0; i < CHUNK_STAGES; ++i) {
+      mbar_init(&B.kv_full[i], 1);
+      mbar_init(&B.kv_free[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B.s_full[i], 1);
+      mbar_init(&B.p_full[i], 4);
+      mbar_init(&B.pv_done[i], 1);
+      mbar_init(&B.o_free[i], 4);
+    }
+    mbar_init(&B.merge_full, 4);
+    B.abort_flag = 0;
+    B.any = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&B.tmem, 512);
+    tmem_relinquish();
+  }
+  if (warp == 10 && lane == 0) {
+    tma_prefetch_desc(&q_big);
+    tma_prefetch_desc(&q_small);
+    tma_prefetch_desc(&kv_map);
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // ---- the call's total cost and the first block of this CTA's range
+  const int per = (a.n_seqs + CHUNK_THREADS - 1) / CHUNK_THREADS;
+  const int i0 = min(tid * per, a.n_seqs), i1 = min(i0 + per, a.n_seqs);
+  long long mine = 0;
+  for (int i = i0; i < i1; ++i) mine += chunk_head_cost(chunk_seq(a, i), bt) * a.nkv;
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) B.scan[warp] = incl;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  long long total = 0;
+  for (int i = 0; i < CHUNK_THREADS / 32; ++i) {
+    if (i < warp) incl += B.scan[i];
+    total += B.scan[i];
+  }
+  const long long lo = chunk_bound(total, cta, grid), hi = chunk_bound(total, cta + 1, grid);
+  if (lo < hi && incl - mine <= lo && lo < incl) {
+    long long base = incl - mine;
+    int i = i0;
+    ChunkSeq s;
+    long long head_cost;
+    while (true) {
+      s = chunk_seq(a, i);
+      head_cost = chunk_head_cost(s, bt);
+      if (lo < base + head_cost * a.nkv) break;
+      base += head_cost * a.nkv;
+      ++i;
+    }
+    const int g = static_cast<int>((lo - base) / head_cost);
+    base += g * head_cost;
+    int k = 0;
+    while (lo >= base + chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST) {
+      base += chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST;
+      ++k;
+    }
+    B.i = i;
+    B.g = g;
+    B.k = k;
+    B.base = base;
+    B.any = 1;
+  }
+  __syncthreads();
+  const uint32_t tmem = B.tmem;
+  volatile int* abort_flag = &B.abort_flag;
+  ChunkWalk w;
+  bool more = B.any != 0;
+  if (more) {
+    w.i = B.i;
+    w.g = B.g;
+    w.k = B.k;
+    w.base = B.base;
+    w.lo = lo;
+    w.hi = hi;
+    w.s = chunk_seq(a, w.i);
+    w.nb = (w.s.n + bt - 1) / bt;
+    more = chunk_fit(a, w, bt);
+  }
+  ChunkMeta* meta = reinterpret_cast<ChunkMeta*>(a.ws + static_cast<size_t>(cta) * 64);
+  if (tid == 0) meta->state = 0;
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");  // 256 x 208 + 128 x 88 = the launch's 384 x 168
+    // ================================================================ softmax and output
+    const int grp = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + grp * 128 + lanes, t_o = tmem + 256 + grp * 128 + lanes;
+    uint32_t n_s = 0, n_pv = 0, n_merge = 0, n_unit = 0;  // tiles of this group, merges and blocks so far
+    for (; more; more = chunk_next(a, w, bt), ++n_unit) {
+      const int tok0 = w.k * bt, ntok = min(w.s.n - tok0, bt), nt = w.t1 - w.t0;
+      const bool pair = ntok > T_tok;
+      const int tok = (pair ? grp * T_tok : 0) + row / group;
+      const bool valid = row < T_tok * group && tok < ntok;
+      const int pos = w.s.len - w.s.n + tok0 + tok;  // the row's position
+      const bool live = __any_sync(0xffffffffu, valid);
+      const int step = pair ? 1 : 2, first = pair ? 0 : grp;
+      float m = -INFINITY, l = 0.0f;
+      for (int j = first; j < nt; j += step) {
+        if (!chunk_wait(&B.s_full[grp], n_s & 1, abort_flag)) goto softmax_out;
+        ++n_s;
+        tc_fence_after();
+        // (not before this block's first S: only then is the barrier's previous phase over)
+        if (pair && grp == 0 && j == 0 && lane == 0) mbar_arrive(&B.q_free);
+        if (live) {
+          float s[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_x32(t_s + c * 32, s + c * 32);
+          tmem_wait_ld();
+          if (a.negate) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c) s[c] = -s[c];
+          }
+          const int limit = valid ? pos - (w.t0 + j) * CHUNK_KT : -1;  // last key of the tile that the row sees
+          if (__any_sync(0xffffffffu, limit < CHUNK_KT - 1)) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c) s[c] = c <= limit ? s[c] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int c = 4; c < 128; c += 4) {
+            mx[0] = fmaxf(mx[0], s[c]);
+            mx[1] = fmaxf(mx[1], s[c + 1]);
+            mx[2] = fmaxf(mx[2], s[c + 2]);
+            mx[3] = fmaxf(mx[3], s[c + 3]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          const bool raise = top > m + CHUNK_RESCALE;
+          if (j == first) {
+            m = top;
+          } else if (__any_sync(0xffffffffu, raise)) {
+            // O holds the sums under the old maximum: bring it under the new one
+            if (!chunk_wait(&B.pv_done[grp], (n_pv - 1) & 1, abort_flag)) goto softmax_out;
+            tc_fence_after();
+            const float f = raise ? ex2(m - top) : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld_x32(t_o + c * 32, reinterpret_cast<float*>(o));
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st_x32(t_o + c * 32, o);
+            }
+            tmem_wait_st();
+            l *= f;
+            if (raise) m = top;
+          }
+          const float base = m == -INFINITY ? 0.0f : m;
+          float sum[4] = {};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t p[32];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              const int x = h * 64 + c * 2;
+              const float p0 = ex2(fmaf(s[x], a.scale_log2, -base)), p1 = ex2(fmaf(s[x + 1], a.scale_log2, -base));
+              const float p2 = ex2(fmaf(s[x + 2], a.scale_log2, -base)), p3 = ex2(fmaf(s[x + 3], a.scale_log2, -base));
+              sum[0] += p0;
+              sum[1] += p1;
+              sum[2] += p2;
+              sum[3] += p3;
+              p[c] = TT::from_f32(p0, p1);
+              p[c + 1] = TT::from_f32(p2, p3);
+            }
+            tmem_st_x32(t_s + h * 32, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        ++n_pv;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.p_full[grp]);
+      }
+      if (l != l) m = l;  // a score that is not a number must show in every join
+      // ---- the block's end
+      const bool had = first < nt;  // this group had tiles
+      if (had) {
+        if (!chunk_wait(&B.pv_done[grp], (n_pv - 1) & 1, abort_flag)) goto softmax_out;
+        tc_fence_after();
+      }
+      const bool merge = !pair && nt > 1;
+      if (grp == 1 && !pair) {
+        if (had) {
+          // O goes where Q was: the other group's products may still read it
+          if (!chunk_wait(&B.q_done, n_unit & 1, abort_flag)) goto softmax_out;
+          if (live) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float o[32];
+              tmem_ld_x32(t_o + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) sm_o[(c * 32 + x) * 128 + row] = o[x];
+            }
+            sm_ml[row] = m;
+            sm_ml[128 + row] = l;
+          }
+          tc_fence_before();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&B.o_free[1]);
+            mbar_arrive(&B.merge_full);
+          }
+        }
+        continue;
+      }
+      // a range in which the row saw nothing (m = -inf) is left out of every sum: its O may be anything
+      bool has0 = m != -INFINITY, has1 = false;
+      float f0 = 1.0f, f1 = 0.0f;
+      if (merge) {
+        if (!chunk_wait(&B.merge_full, n_merge & 1, abort_flag)) goto softmax_out;
+        ++n_merge;
+        if (live) {
+          const float m1 = sm_ml[row], l1 = sm_ml[128 + row], top = fmaxf(m, m1);
+          has1 = m1 != -INFINITY;
+          f0 = has0 ? ex2(m - top) : 0.0f;
+          f1 = has1 ? ex2(m1 - top) : 0.0f;
+          l = (has0 ? l * f0 : 0.0f) + (has1 ? l1 * f1 : 0.0f);
+          if (l != l) m = l;
+          else m = top;
+        }
+      }
+      const bool whole = w.t0 == 0 && w.t1 == w.nt;
+      const bool seen = pos >= 0;
+      const int out_row = w.s.row0 + tok0 + tok, qhead = w.g * group + row % group;
+      const int prow = (pair ? grp * 128 : 0) + row;
+      float* part = chunk_part(a, grid, w.t0 == 0 ? 2 * cta + 1 : 2 * cta);
+      float bad = 0.0f;
+      if (live) {
+        const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
+        T* out = static_cast<T*>(a.out) + static_cast<size_t>(out_row) * a.out_ld + qhead * CHUNK_DIM;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          tmem_ld_x32(t_o + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            float v = has0 ? o[x] * f0 : 0.0f;
+            if (has1) v += sm_o[(c * 32 + x) * 128 + row] * f1;
+            v = seen ? v * inv : 0.0f;
+            bad = fmaf(v, 0.0f, bad);  // NaN once a value is not finite
+            o[x] = v;
+          }
+          if (valid && whole) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+              uint4 v;
+              v.x = TT::from_f32(o[x], o[x + 1]);
+              v.y = TT::from_f32(o[x + 2], o[x + 3]);
+              v.z = TT::from_f32(o[x + 4], o[x + 5]);
+              v.w = TT::from_f32(o[x + 6], o[x + 7]);
+              *reinterpret_cast<uint4*>(out + c * 32 + x) = v;
+            }
+          } else if (valid) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) part[(c * 32 + x) * CHUNK_PART_ROWS + prow] = o[x];
+          }
+        }
+        if (valid && !whole) {
+          part[CHUNK_DIM * CHUNK_PART_ROWS + prow] = m;
+          part[(CHUNK_DIM + 1) * CHUNK_PART_ROWS + prow] = l;
+        }
+      }
+      tc_fence_before();
+      if (merge) fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&B.o_free[grp]);
+        if (!pair) mbar_arrive(&B.q_free);
+      }
+      // rows that came out not finite, one after the other
+      for (unsigned again = __ballot_sync(0xffffffffu, valid && !(bad == 0.0f)); again; again &= again - 1) {
+        const int src = __ffs(again) - 1;
+        const int r_row = __shfl_sync(0xffffffffu, out_row, src), r_head = __shfl_sync(0xffffffffu, qhead, src);
+        const int r_pos = __shfl_sync(0xffffffffu, pos, src), r_prow = __shfl_sync(0xffffffffu, prow, src);
+        float rm, rl;
+        float4 o;
+        chunk_row<BF16>(a, w.s, r_row, r_head, w.t0 * CHUNK_KT, min(w.t1 * CHUNK_KT, r_pos + 1), rm, rl, o);
+        if (whole) {
+          const float inv = 1.0f / rl;
+          uint2 v;
+          v.x = TT::from_f32(o.x * inv, o.y * inv);
+          v.y = TT::from_f32(o.z * inv, o.w * inv);
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(r_row) * a.out_ld + r_head * CHUNK_DIM +
+                                    lane * 4) = v;
+        } else {
+          part[(lane * 4) * CHUNK_PART_ROWS + r_prow] = o.x;
+          part[(lane * 4 + 1) * CHUNK_PART_ROWS + r_prow] = o.y;
+          part[(lane * 4 + 2) * CHUNK_PART_ROWS + r_prow] = o.z;
+          part[(lane * 4 + 3) * CHUNK_PART_ROWS + r_prow] = o.w;
+          if (lane == 0) {
+            part[CHUNK_DIM * CHUNK_PART_ROWS + r_prow] = rm;
+            part[(CHUNK_DIM + 1) * CHUNK_PART_ROWS + r_prow] = rl;
+          }
+        }
+      }
+      if (!whole && w.t0 == 0 && tid == 0) {
+        meta->row0 = w.s.row0 + tok0;
+        meta->ntok = ntok;
+        meta->head = w.g;
+        meta->nt = w.nt;
+        meta->pos0 = w.s.len - w.s.n + tok0;
+        meta->base = w.base;
+        meta->total = total;
+        meta->state = 1;
+      }
+    }
+  softmax_out:;
+  } else if (warp < 10) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ================================================================ MMA issue
+    const int grp = warp - 8;
+    const uint32_t t_s = tmem + grp * 128, t_o = tmem + 256 + grp * 128;
+    constexpr uint32_t id_qk = chunk_idesc<BF16>(false), id_pv = chunk_idesc<BF16>(true);
+    uint32_t n_unit = 0, n_tile = 0, n_out = 0, ring = 0;
+    // Both issuers wait for every ring position, in order, and both release it: by the MMAs that read it, or, for a
+    // stage of a one-tile block that only the other group reads, at once.  So neither can miss a phase.
+    uint32_t landed = 0;
+    auto ready = [&](uint32_t upto, bool pass) {
+      for (; landed < upto; ++landed) {
+        const uint32_t st = landed % CHUNK_STAGES;
+        if (!chunk_wait(&B.kv_full[st], (landed / CHUNK_STAGES) & 1, abort_flag)) return false;
+        if (pass && lane == 0) mbar_arrive(&B.kv_free[st]);
+      }
+      return true;
+    };
+    auto mine = [&](uint32_t it, bool pair) { return ready(it, !pair) && ready(it + 1, false); };
+    for (; more; more = chunk_next(a, w, bt)) {
+      const int tok0 = w.k * bt, ntok = min(w.s.n - tok0, bt), nt = w.t1 - w.t0;
+      const bool pair = ntok > T_tok;
+      const int step = pair ? 1 : 2, first = pair ? 0 : grp;
+      const int end = w.s.len - w.s.n + tok0 + ntok;  // positions the block sees
+      const uint32_t q_addr = smem_u32(sm_q) + (pair ? grp * CHUNK_STAGE_BYTES : 0);
+      if (!chunk_wait(&B.q_full, n_unit & 1, abort_flag)) goto mma_out;
+      if (first >= nt) {  // a one-tile block of one key tile: nothing for the second group
+        if (lane == 0) {
+          mbar_arrive(&B.q_free);
+          mbar_arrive(&B.q_done);
+        }
+      } else {
+        for (int j = first - step; j < nt; j += step) {
+          if (j >= 0) {
+            const uint32_t it = ring + chunk_v_at(j, nt), st = it % CHUNK_STAGES;
+            if (!mine(it, pair)) goto mma_out;
+            uint8_t* v = sm_kv + st * CHUNK_STAGE_BYTES;
+            const int held = end - (w.t0 + j) * CHUNK_KT;  // positions of this tile that the block sees
+            if (held < CHUNK_KT) {
+              // both issuers may clear the same rows: the same zeros
+              for (int x = max(held, 0) * 8 + lane; x < CHUNK_KT * 8; x += 32) {
+                reinterpret_cast<uint4*>(v)[x] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(v + CHUNK_HALF_BYTES)[x] = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+            if (j == first) {
+              if (n_out && !chunk_wait(&B.o_free[grp], (n_out - 1) & 1, abort_flag)) goto mma_out;
+              ++n_out;
+            }
+            if (!chunk_wait(&B.p_full[grp], n_tile & 1, abort_flag)) goto mma_out;
+            ++n_tile;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint64_t d = smem_desc_v(smem_u32(v));
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                umma_f16_ts(t_o, t_s + x * 8, d + x * (2048 >> 4), id_pv, (j > first || x > 0) ? 1u : 0u);
+              umma_commit(&B.pv_done[grp]);
+              umma_commit(&B.kv_free[st]);
+            }
+            __syncwarp();
+          }
+          const int jn = j + step;
+          if (jn < nt) {
+            const uint32_t it = ring + chunk_k_at(jn), st = it % CHUNK_STAGES;
+            if (!mine(it, pair)) goto mma_out;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint64_t dq = smem_desc_sw128(q_addr), dk = smem_desc_sw128(smem_u32(sm_kv + st * CHUNK_STAGE_BYTES));
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const uint32_t off = ((x >> 2) * CHUNK_HALF_BYTES + (x & 3) * 32) >> 4;
+                umma_f16_ss(t_s, dq + off, dk + off, id_qk, x > 0 ? 1u : 0u);
+              }
+              umma_commit(&B.s_full[grp]);
+              umma_commit(&B.kv_free[st]);
+              if (jn + step >= nt) {
+                umma_commit(&B.q_free);
+                umma_commit(&B.q_done);
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+      ++n_unit;
+      ring += 2 * nt;
+      if (!ready(ring, !pair)) goto mma_out;
+    }
+  mma_out:;
+  } else if (warp == 10) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ================================================================ copies
+    uint32_t n_unit = 0, ring = 0;
+    for (; more; more = chunk_next(a, w, bt)) {
+      const int tok0 = w.k * bt, ntok = min(w.s.n - tok0, bt), nt = w.t1 - w.t0;
+      const bool pair = ntok > T_tok;
+      const int end = w.s.len - w.s.n + tok0 + ntok;
+      if (n_unit && !chunk_wait(&B.q_free, (n_unit - 1) & 1, abort_flag)) goto copy_out;
+      if (lane == 0) {
+        const bool small = ntok <= 8;
+        const int tiles = pair ? 2 : 1;
+        mbar_arrive_expect_tx(&B.q_full, tiles * 2 * (small ? 8 : T_tok) * group * 128);
+        for (int x = 0; x < tiles; ++x)
+          for (int h = 0; h < 2; ++h)
+            tma_load_4d(sm_q + x * CHUNK_STAGE_BYTES + h * CHUNK_HALF_BYTES, small ? &q_small : &q_big, &B.q_full, 0,
+                        w.g * group, w.s.row0 + tok0 + x * T_tok, h);
+      }
+      __syncwarp();
+      const int pages = min((max(end, 0) + CHUNK_PAGE - 1) / CHUNK_PAGE, 2 * w.t1);  // of the range, from page 0 on
+      int page_of = 0, from = -1;
+      for (int x = 0; x < 2 * nt; ++x) {
+        // ring order: K0 K1 V0 K2 V1 ...
+        const bool is_v = nt == 1 ? x == 1 : x == 2 * nt - 1 || (x > 1 && (x & 1) == 0);
+        const int j = x == 2 * nt - 1 ? nt - 1 : is_v ? (x - 2) / 2 : (x + 1) / 2;
+        const int p0 = 2 * (w.t0 + j), have = min(2, pages - p0);
+        if (from < 0 || p0 < from || p0 + 2 > from + 32) {  // page ids, 32 at a time
+          from = is_v ? p0 : max(p0 - 4, 0);
+          page_of = from + lane < pages ? a.page_table[static_cast<size_t>(w.s.slot) * a.max_pages + from + lane] : -1;
+        }
+        const uint32_t it = ring + x, st = it % CHUNK_STAGES;
+        if (it >= CHUNK_STAGES && !chunk_wait(&B.kv_free[st], (it / CHUNK_STAGES - 1) & 1, abort_flag)) goto copy_out;
+        const int pg0 = __shfl_sync(0xffffffffu, page_of, (p0 - from) & 31), pg1 = __shfl_sync(0xffffffffu, page_of, (p0 + 1 - from) & 31);
+        if (lane == 0) {
+          uint8_t* dst = sm_kv + st * CHUNK_STAGE_BYTES;
+          if (have > 0) mbar_arrive_expect_tx(&B.kv_full[st], have * CHUNK_PAGE * CHUNK_DIM * 2);
+          else mbar_arrive(&B.kv_full[st]);
+          for (int y = 0; y < have; ++y) {
+            const int page = y ? pg1 : pg0;
+            // a page outside the pool reads as zeros: rows behind the map's last
+            const int r = page < 0 || page >= a.pool_pages
+                              ? a.pool_pages * a.layers * 2 * a.nkv * CHUNK_PAGE
+                              : (((page * a.layers + a.layer) * 2 + (is_v ? 1 : 0)) * a.nkv + w.g) * CHUNK_PAGE;
+            for (int h = 0; h < 2; ++h)
+              tma_load_3d(dst + h * CHUNK_HALF_BYTES + y * (CHUNK_PAGE * 128), &kv_map, &B.kv_full[st], 0, r, h);
+          }
+        }
+        __syncwarp();
+      }
+      ++n_unit;
+      ring += 2 * nt;
+    }
+  copy_out:
+    if (*abort_flag && lane == 0) {
+      // copies still in flight land before the shared memory is given back: the newest of each stage, bounded
+      const uint64_t t0 = globaltimer();
+      for (int st = 0; st < CHUNK_STAGES; ++st)
+        for (uint32_t x = 0; x < 2; ++x)
+          while (!mbar_try_wait(&B.kv_full[st], x) && globaltimer() - t0 < 20000000ull) {
+          }
+      for (uint32_t x = 0; x < 2; ++x)
+        while (!mbar_try_wait(&B.q_full, x) && globaltimer() - t0 < 40000000ull) {
+        }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && B.abort_flag) meta->state = 2;
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+// Joins the partials of the block that CTA blockIdx.x began and others went on with; blockIdx.y takes
+// 32 rows of it, a thread one row and 16 dims.
+template <bool BF16>
+__global__ void __launch_bounds__(256) attention_chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int grid) {
+  using TT = ChunkType<BF16>;
+  using T = typename TT::T;
+  griddep_wait();
+  griddep_launch_dependents();
+  const ChunkMeta* meta = reinterpret_cast<const ChunkMeta*>(a.ws + static_cast<size_t>(blockIdx.x) * 64);
+  if (meta->state != 1) return;
+  const int group = a.nq / a.nkv, T_tok = chunk_tile_tokens(group);
+  const int prow = blockIdx.y * 32 + (threadIdx.x & 31), col = (threadIdx.x >> 5) * 16;
+  const int tok = (prow >> 7) * T_tok + (prow & 127) / group, head = meta->head * group + (prow & 127) % group;
+  if ((prow & 127) >= T_tok * group || tok >= meta->ntok) return;
+  const int nt = meta->nt;
+  const long long base = meta->base, total = meta->total;
+  float top = -INFINITY;
+  for (int pass = 0; pass < 2; ++pass) {
+    float l = 0.0f, o[16] = {};
+    for (int c = blockIdx.x, end = 0; end < nt && c < grid; ++c) {
+      const int t0 = chunk_cut(chunk_bound(total, c, grid), base, nt), t1 = chunk_cut(chunk_bound(total, c + 1, grid), base, nt);
+      end = t1;
+      if (t1 <= t0) continue;
+      const float* part = chunk_part(a, grid, c == static_cast<int>(blockIdx.x) ? 2 * c + 1 : 2 * c) + prow;
+      const float m = part[CHUNK_DIM * CHUNK_PART_ROWS];
+      if (pass == 0) {
+        top = fmaxf(top, m);
+      } else if (m != -INFINITY) {
+        const float f = ex2(m - top);
+        l += part[(CHUNK_DIM + 1) * CHUNK_PART_ROWS] * f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[x] += part[(col + x) * CHUNK_PART_ROWS] * f;
+      }
+    }
+    if (pass == 0) continue;
+    const float inv = meta->pos0 + tok < 0 ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + static_cast<size_t>(meta->row0 + tok) * a.out_ld + head * CHUNK_DIM + col;
+#pragma unroll
+    for (int x = 0; x < 16; x += 8) {
+      uint4 v;
+      v.x = TT::from_f32(o[x] * inv, o[x + 1] * inv);
+      v.y = TT::from_f32(o[x + 2] * inv, o[x + 3] * inv);
+      v.z = TT::from_f32(o[x + 4] * inv, o[x + 5] * inv);
+      v.w = TT::from_f32(o[x + 6] * inv, o[x + 7] * inv);
+      *reinterpret_cast<uint4*>(out + x) = v;
+    }
+  }
 }
 
 }  // namespace qasr

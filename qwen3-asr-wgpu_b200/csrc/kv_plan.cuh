@@ -196,8 +196,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
     else
       a.page_table[line + ((held[lo] + 63) >> 6) + (p - page0[lo])] = a.free_pages[free_count - 1 - p];
   }
-  if (RELEASE) return;
-  for (int r = gt; r < static_cast<int>(rows); r += threads) {
+  for (int r = gt; !RELEASE && r < static_cast<int>(rows); r += threads) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;

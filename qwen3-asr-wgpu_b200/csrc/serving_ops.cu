@@ -7,6 +7,7 @@
 
 #include <cmath>
 #include <cstdio>
+#include <cstring>
 #include <mutex>
 #include <string>
 
@@ -71,6 +72,44 @@ cudaError_t plan_attrs(int device) noexcept {
     return cudaErrorUnknown;
   }
   return result[device];
+}
+
+int sm_count(int device) noexcept {
+  int n = 0;
+  if (device < 0 || device >= kMaxDevices ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return -1;
+  return n;
+}
+
+cudaError_t chunk_attrs(int device) noexcept {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t result[kMaxDevices] = {};
+  try {
+    std::call_once(once[device], [device] {
+      cudaError_t e =
+          cudaFuncSetAttribute(attention_chunk_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_SMEM);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attention_chunk_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_SMEM);
+      result[device] = e;
+    });
+  } catch (...) {
+    return cudaErrorUnknown;
+  }
+  return result[device];
+}
+
+bool encode_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                const cuuint32_t* box, bool swizzle) noexcept {
+  try {
+    const EncodeTiledFn fn = encode_fn(nullptr);
+    const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+    return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), dims, strides, box, step,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  } catch (...) {
+    return false;
+  }
 }
 
 template <bool RELEASE>
@@ -139,7 +178,8 @@ qasr_status qasr_kernel_kv_release(int device, void* stream, const int* seq_slot
 }
 
 int64_t qasr_kernel_attention_chunk_workspace(int device) {
-  return device < 0 || device >= kMaxDevices ? -1 : 256;
+  const int sms = sm_count(device);
+  return sms <= 0 ? -1 : chunk_ws_bytes(sms);
 }
 
 qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, const void* q, int q_ld, void* out,
@@ -157,17 +197,60 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
     return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad chunk attention arguments");
   DeviceScope dev(device);
   if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
-  if (ws_bytes < qasr_kernel_attention_chunk_workspace(device))
+  const int grid = sm_count(device);
+  if (grid <= 0) return op_err(err, errlen, QASR_ERR_DEVICE, "device attributes");
+  if (ws_bytes < chunk_ws_bytes(grid))
     return op_err(err, errlen, QASR_ERR_CAPACITY, "chunk attention workspace too small");
-  ChunkArgs a{q, q_ld, out, out_ld, rows, kv_pool, pool_pages, page_table, max_slots, max_pages, layers, nq, nkv, layer,
-              seq_slot, cu_rows, kv_len, n_seqs, scale * 1.4426950408889634f};
-  const long long units = static_cast<long long>(rows) * nq;
-  if ((units + 7) / 8 > 0x7fffffff) return op_err(err, errlen, QASR_ERR_CAPACITY, "too many rows");
-  const dim3 grid(static_cast<unsigned>((units + 7) / 8));
+  cudaError_t e = chunk_attrs(device);
+  if (e != cudaSuccess) return op_cuda(err, errlen, e, "kernel attributes");
+  const int group = nq / nkv;
+  const uint64_t kv_rows = static_cast<uint64_t>(pool_pages) * layers * 2 * nkv * CHUNK_PAGE;
+  // Q as {64 dims, heads, rows, 2 halves}: a box is one half of a group's heads of some rows, in the order in which
+  // a row tile packs them, under the tensor core's 128-byte swizzle.  The cache as {64 dims, rows, 2
+  // halves}: a box is one half of a page, copied as it is (its rows are swizzled already).
+  CUtensorMap q_big, q_small, kv_map;
+  const cuuint64_t q_dims[4] = {64, static_cast<cuuint64_t>(nq), static_cast<cuuint64_t>(rows), 2};
+  const cuuint64_t q_strides[3] = {CHUNK_DIM * 2, static_cast<cuuint64_t>(q_ld) * 2, 128};
+  const cuuint32_t big[4] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(chunk_tile_tokens(group)), 1};
+  const cuuint32_t small[4] = {64, static_cast<cuuint32_t>(group), 8, 1};
+  const cuuint64_t kv_dims[3] = {64, kv_rows, 2}, kv_strides[2] = {CHUNK_DIM * 2, 128};
+  const cuuint32_t kv_box[3] = {64, CHUNK_PAGE, 1};
+  if (!encode_map(&q_big, q, 4, q_dims, q_strides, big, true) || !encode_map(&q_small, q, 4, q_dims, q_strides, small, true) ||
+      !encode_map(&kv_map, kv_pool, 3, kv_dims, kv_strides, kv_box, false))
+    return op_err(err, errlen, QASR_ERR_DEVICE, "chunk attention tensor maps");
+  // a scale of 0 becomes a tiny one: masked scores stay -inf under it, and every other score still counts alike
+  const float s2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+  const ChunkArgs a{q, q_ld, out, out_ld, rows, kv_pool, pool_pages, page_table, max_slots, max_pages, layers, nq, nkv,
+                    layer, seq_slot, cu_rows, kv_len, n_seqs, s2, scale < 0.0f, static_cast<uint8_t*>(ws)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = type == QASR_TYPE_BF16 ? launch_k(attention_chunk_rows_kernel<true>, grid, dim3(256), 0, st, true, a)
-                                               : launch_k(attention_chunk_rows_kernel<false>, grid, dim3(256), 0, st, true, a);
-  return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "chunk attention launch");
+  const bool bf = type == QASR_TYPE_BF16;
+  e = bf ? launch_k(attention_chunk_kernel<true>, dim3(grid), dim3(CHUNK_THREADS), CHUNK_SMEM, st, true, q_big, q_small, kv_map, a)
+         : launch_k(attention_chunk_kernel<false>, dim3(grid), dim3(CHUNK_THREADS), CHUNK_SMEM, st, true, q_big, q_small, kv_map, a);
+  if (e != cudaSuccess) return op_cuda(err, errlen, e, "chunk attention launch");
+  const dim3 cgrid(grid, CHUNK_PART_ROWS / 32);
+  e = bf ? launch_k(attention_chunk_combine_kernel<true>, cgrid, dim3(256), 0, st, true, a, grid)
+         : launch_k(attention_chunk_combine_kernel<false>, cgrid, dim3(256), 0, st, true, a, grid);
+  return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "chunk attention combine launch");
+}
+
+qasr_status qasr_kernel_attention_chunk_check(int device, void* stream, const void* ws, char* err, int errlen) {
+  if (!ws || misaligned(ws, 256)) return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad chunk attention workspace");
+  DeviceScope dev(device);
+  if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
+  const int grid = sm_count(device);
+  static_assert(sizeof(ChunkMeta) <= 64, "one 64-byte line per CTA");
+  if (grid <= 0 || grid > 512) return op_err(err, errlen, QASR_ERR_DEVICE, "device attributes");
+  alignas(8) unsigned char lines[512 * 64];
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyAsync(lines, ws, static_cast<size_t>(grid) * 64, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return op_cuda(err, errlen, e, "chunk attention status");
+  for (int c = 0; c < grid; ++c) {
+    int state;
+    std::memcpy(&state, lines + c * 64, sizeof state);
+    if (state == 2) return op_err(err, errlen, QASR_ERR_DEVICE_TIMEOUT, "a device-side wait of the chunk attention timed out");
+  }
+  return QASR_OK;
 }
 
 int64_t qasr_kernel_w4_packed_bytes(int n_out, int k, int group, int has_zero) {

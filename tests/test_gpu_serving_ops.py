@@ -334,8 +334,9 @@ HEADS = [(16, 8), (8, 8), (16, 2), (12, 4), (16, 1), (5, 1)]
 def test_chunk_attention_matches_the_formula(qasr, cuda_device, lens, nq, nkv, dtype):
     import torch
     c = Chunks(torch, lens, nq=nq, nkv=nkv, dtype=dtype, seed=len(lens) + nq)
-    out = c.run(qasr)
-    torch.cuda.synchronize()
+    ws = c.workspace(qasr)
+    out = c.run(qasr, ws=ws)
+    qasr.kernel_attention_chunk_check(0, _stream(torch), ws[0].data_ptr())  # waits for the stream
     c.check(out)
 
 

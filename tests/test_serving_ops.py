@@ -59,6 +59,13 @@ def test_attention_chunk_refuses_bad_arguments(qasr, change):
     assert e.value.status == 1 and "chunk attention" in str(e.value)
 
 
+def test_attention_chunk_check_refuses_bad_workspaces(qasr):
+    for ptr in (0, A + 8):
+        with pytest.raises(qasr.DecoderError) as e:
+            qasr.kernel_attention_chunk_check(0, 0, ptr)
+        assert e.value.status == 1
+
+
 def test_devices_out_of_range_are_refused(qasr):
     with pytest.raises(qasr.DecoderError):
         qasr.kernel_attention_chunk_workspace(-1)
