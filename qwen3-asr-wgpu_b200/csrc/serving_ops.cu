@@ -148,6 +148,24 @@ bool bad_w4_sizes(int n_out, int k, int group) {
          n_out > (1 << 30) || k > (1 << 30);
 }
 
+template <bool BF16, bool ZERO, bool G32, int MT, int NT>
+cudaError_t launch_w4_tiles(const W4Args& a, cudaStream_t st) {
+  return launch_k(gemv_w4_kernel<BF16, ZERO, G32, MT, NT>, dim3((a.n_out + 16 * MT - 1) / (16 * MT)), dim3(W4_THREADS), 0, st,
+                  true, a);
+}
+template <bool BF16, bool ZERO, bool G32>
+cudaError_t launch_w4_rows(const W4Args& a, cudaStream_t st) {
+  if (a.rows <= 8) return launch_w4_tiles<BF16, ZERO, G32, 1, 1>(a, st);
+  if (a.rows <= 16) return launch_w4_tiles<BF16, ZERO, G32, 1, 2>(a, st);
+  if (a.rows <= 32) return launch_w4_tiles<BF16, ZERO, G32, 1, 4>(a, st);
+  return launch_w4_tiles<BF16, ZERO, G32, 1, 8>(a, st);
+}
+template <bool BF16>
+cudaError_t launch_w4(const W4Args& a, bool zero, cudaStream_t st) {
+  if (a.group_log2 == 5) return zero ? launch_w4_rows<BF16, true, true>(a, st) : launch_w4_rows<BF16, false, true>(a, st);
+  return zero ? launch_w4_rows<BF16, true, false>(a, st) : launch_w4_rows<BF16, false, false>(a, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -279,13 +297,8 @@ qasr_status qasr_kernel_gemv_w4(int device, void* stream, int type, const void* 
   if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
   const W4Args a{static_cast<const uint8_t*>(packed), n_out, k, group == 32 ? 5 : group == 64 ? 6 : 7, x, ldx, rows, out,
                  ldo, accumulate != 0};
-  const dim3 grid((n_out + 15) / 16);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool bf = type == QASR_TYPE_BF16;
-  const cudaError_t e = bf ? (has_zero ? launch_k(gemv_w4_kernel<true, true>, grid, dim3(W4_THREADS), 0, st, true, a)
-                                       : launch_k(gemv_w4_kernel<true, false>, grid, dim3(W4_THREADS), 0, st, true, a))
-                           : (has_zero ? launch_k(gemv_w4_kernel<false, true>, grid, dim3(W4_THREADS), 0, st, true, a)
-                                       : launch_k(gemv_w4_kernel<false, false>, grid, dim3(W4_THREADS), 0, st, true, a));
+  const cudaError_t e = type == QASR_TYPE_BF16 ? launch_w4<true>(a, has_zero != 0, st) : launch_w4<false>(a, has_zero != 0, st);
   return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "w4 gemv launch");
 }
 
