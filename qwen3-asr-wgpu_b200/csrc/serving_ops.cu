@@ -148,22 +148,61 @@ bool bad_w4_sizes(int n_out, int k, int group) {
          n_out > (1 << 30) || k > (1 << 30);
 }
 
-template <bool BF16, bool ZERO, bool G32, int MT, int NT>
-cudaError_t launch_w4_tiles(const W4Args& a, cudaStream_t st) {
-  return launch_k(gemv_w4_kernel<BF16, ZERO, G32, MT, NT>, dim3((a.n_out + 16 * MT - 1) / (16 * MT)), dim3(W4_THREADS), 0, st,
-                  true, a);
+template <bool BF16, bool ZERO, int GS, int NT>
+cudaError_t launch_w4_kernel(W4Args a, int device, int sms, cudaStream_t st) {
+  using P = W4Plan<ZERO, GS, NT>;
+  static_assert(P::slots >= 2 && P::slots * W4_WARPS * 8 <= P::bars_bytes - 16, "a ring has two slots at least");
+  const auto kernel = gemv_w4_kernel<BF16, ZERO, GS, NT>;
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t ready[kMaxDevices] = {};
+  std::call_once(once[device], [kernel, device] {
+    ready[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::smem);
+  });
+  if (ready[device] != cudaSuccess) return ready[device];
+  const W4Layout L = w4_layout(a.n_out, a.k, 128 / GS, ZERO);
+  a.wk_log2 = 3;
+  while ((1 << a.wk_log2) > L.units) --a.wk_log2;
+  // Few row tiles: two or four CTAs share each, as long as they fit the SMs and every warp still has a unit.
+  a.cluster = 1;
+  while (a.cluster < W4_MAX_CLUSTER && L.tiles * a.cluster * 2 <= sms && L.units >= 16 * a.cluster) a.cluster *= 2;
+  const int per_cta = W4_WARPS >> a.wk_log2;
+  const int groups = (L.tiles + per_cta - 1) / per_cta;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.cluster > 1 ? groups * a.cluster : std::min(groups, sms * P::per_sm));
+  cfg.blockDim = dim3(W4_THREADS);
+  cfg.dynamicSmemBytes = P::smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
-template <bool BF16, bool ZERO, bool G32>
-cudaError_t launch_w4_rows(const W4Args& a, cudaStream_t st) {
-  if (a.rows <= 8) return launch_w4_tiles<BF16, ZERO, G32, 1, 1>(a, st);
-  if (a.rows <= 16) return launch_w4_tiles<BF16, ZERO, G32, 1, 2>(a, st);
-  if (a.rows <= 32) return launch_w4_tiles<BF16, ZERO, G32, 1, 4>(a, st);
-  return launch_w4_tiles<BF16, ZERO, G32, 1, 8>(a, st);
+template <bool BF16, bool ZERO, int GS>
+cudaError_t launch_w4_rows(const W4Args& a, int device, int sms, cudaStream_t st) {
+  if (a.rows <= 8) return launch_w4_kernel<BF16, ZERO, GS, 1>(a, device, sms, st);
+  if (a.rows <= 16) return launch_w4_kernel<BF16, ZERO, GS, 2>(a, device, sms, st);
+  if (a.rows <= 32) return launch_w4_kernel<BF16, ZERO, GS, 4>(a, device, sms, st);
+  return launch_w4_kernel<BF16, ZERO, GS, 8>(a, device, sms, st);
 }
 template <bool BF16>
-cudaError_t launch_w4(const W4Args& a, bool zero, cudaStream_t st) {
-  if (a.group_log2 == 5) return zero ? launch_w4_rows<BF16, true, true>(a, st) : launch_w4_rows<BF16, false, true>(a, st);
-  return zero ? launch_w4_rows<BF16, true, false>(a, st) : launch_w4_rows<BF16, false, false>(a, st);
+cudaError_t launch_w4(const W4Args& a, int group, bool zero, int device, int sms, cudaStream_t st) {
+  switch (group) {
+    case 32: return zero ? launch_w4_rows<BF16, true, 4>(a, device, sms, st) : launch_w4_rows<BF16, false, 4>(a, device, sms, st);
+    case 64: return zero ? launch_w4_rows<BF16, true, 2>(a, device, sms, st) : launch_w4_rows<BF16, false, 2>(a, device, sms, st);
+    default: return zero ? launch_w4_rows<BF16, true, 1>(a, device, sms, st) : launch_w4_rows<BF16, false, 1>(a, device, sms, st);
+  }
 }
 
 }  // namespace
@@ -295,10 +334,12 @@ qasr_status qasr_kernel_gemv_w4(int device, void* stream, int type, const void* 
     return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad w4 gemv arguments");
   DeviceScope dev(device);
   if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
-  const W4Args a{static_cast<const uint8_t*>(packed), n_out, k, group == 32 ? 5 : group == 64 ? 6 : 7, x, ldx, rows, out,
-                 ldo, accumulate != 0};
+  const int sms = sm_count(device);
+  if (sms <= 0) return op_err(err, errlen, QASR_ERR_DEVICE, "device attributes");
+  const W4Args a{static_cast<const uint8_t*>(packed), n_out, k, x, ldx, rows, out, ldo, accumulate != 0, 0, 1};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = type == QASR_TYPE_BF16 ? launch_w4<true>(a, has_zero != 0, st) : launch_w4<false>(a, has_zero != 0, st);
+  const cudaError_t e = type == QASR_TYPE_BF16 ? launch_w4<true>(a, group, has_zero != 0, device, sms, st)
+                                               : launch_w4<false>(a, group, has_zero != 0, device, sms, st);
   return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "w4 gemv launch");
 }
 

@@ -77,11 +77,11 @@ def test_devices_out_of_range_are_refused(qasr):
 
 
 def test_w4_packed_bytes(qasr):
-    # codes in 512-byte blocks of 16 rows x 64 columns, 2 bytes of scale and 1 of zero point per row and group
-    assert qasr.kernel_w4_packed_bytes(16, 64, 64) == 512 + 32
-    assert qasr.kernel_w4_packed_bytes(17, 64, 64) == 2 * (512 + 32)
-    assert qasr.kernel_w4_packed_bytes(16, 128, 32, True) == 2 * 512 + 4 * 16 * 3
-    assert qasr.kernel_w4_packed_bytes(1, 96, 32) == 2 * 512 + 4 * 32  # columns 96..127 are padding
+    # codes in 2 KB units of 32 rows x 128 columns, 2 bytes of scale and 1 of zero point per row and group
+    assert qasr.kernel_w4_packed_bytes(32, 128, 128) == 2048 + 64
+    assert qasr.kernel_w4_packed_bytes(33, 128, 128) == 2 * (2048 + 64)
+    assert qasr.kernel_w4_packed_bytes(32, 128, 32, True) == 2048 + 4 * 32 * 3
+    assert qasr.kernel_w4_packed_bytes(1, 96, 32) == 2048 + 4 * 64  # columns 96..127 are padding
     for n_out, k, g in [(0, 64, 64), (-1, 64, 64), (16, 0, 64), (16, 64, 16), (16, 96, 64), (16, 64, 128), (16, 64, 0)]:
         with pytest.raises(qasr.DecoderError):
             qasr.kernel_w4_packed_bytes(n_out, k, g)
