@@ -17,10 +17,13 @@
 // is taken before that rounding.  m is raised, and O rescaled, only when a row's maximum has grown by more than
 // 2^8 (P then stays below 2^8, far inside f16), so the rescaling, a round trip over O, is rare.
 //
-// Roles: warps 0-3 and 4-7 are two softmax groups, one per row tile; warps 8 and 9 issue the MMAs of one
-// group each; warp 10 copies Q and the pages into a ring of 128-position stages.  A block of one row tile only
-// (a decode step, a short chunk) gives its even key tiles to the first group and the odd ones to the second,
-// which then merge, so both always have work.
+// Roles: warps 0-3 and 4-7 are two softmax groups, one per row tile; warp 8 issues the MMAs, the groups' in turn, so
+// that one group's products run under the other's softmax (two issuers, one a group, fall into step: both
+// groups then wait together); warp 9 copies Q and the pages into a ring of 128-position stages; warp 10
+// walks the schedule and hands the others one block after the other through shared memory, which keeps the walk out of
+// their registers.  The second product starts on the first half of P while the second half is computed.  A block of one
+// row tile only (a decode step, a short chunk) gives its even key tiles to the first group and the odd ones to the
+// second, which then merge, so both always have work.
 //
 // Work split: every (request, kv head, block) costs its key tiles plus CHUNK_BLOCK_COST; the costs of the whole call,
 // laid end to end, are cut into one equal range per CTA.  A block that a cut goes through leaves f32
@@ -66,7 +69,7 @@ constexpr int CHUNK_STAGES = 5;
 constexpr int CHUNK_STAGE_BYTES = CHUNK_KT * CHUNK_DIM * 2;
 constexpr int CHUNK_HALF_BYTES = CHUNK_KT * 128;  // 128 rows of one 64-dim half
 constexpr int CHUNK_Q_BYTES = 2 * CHUNK_STAGE_BYTES;
-constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + CHUNK_STAGES * CHUNK_STAGE_BYTES + 1536;
+constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + CHUNK_STAGES * CHUNK_STAGE_BYTES + 2048;
 constexpr int CHUNK_BLOCK_COST = 1;               // a block's Q copy, first and last steps, in key tiles
 constexpr int CHUNK_SNAP = 1;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
@@ -225,6 +228,28 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two f32 at a time
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // Shared-memory descriptor of V as the second operand, MN-major with 128-byte swizzle: 64-dim halves
 // CHUNK_HALF_BYTES apart (LBO), groups of 8 positions 1024 bytes apart (SBO).
 __device__ __forceinline__ uint64_t smem_desc_v(uint32_t smem_addr) {
@@ -259,7 +284,7 @@ __device__ __forceinline__ bool chunk_wait(uint64_t* bar, uint32_t parity, volat
 // One row's (m, l, o) over the positions [t0, t1) without matrix instructions: a warp, lane l holding the dims
 // 4l .. 4l + 3.  For the rows whose tensor core result is not finite.
 template <bool BF16>
-__device__ __noinline__ void chunk_row(const ChunkArgs& a, const ChunkSeq& s, int row, int qhead, int t0, int t1,
+__device__ __noinline__ void chunk_row(const ChunkArgs& a, int slot, int row, int qhead, int t0, int t1,
                                        float& m, float& l, float4& o) {
   using TT = ChunkType<BF16>;
   using T = typename TT::T;
@@ -271,7 +296,7 @@ __device__ __noinline__ void chunk_row(const ChunkArgs& a, const ChunkSeq& s, in
   l = 0.0f;
   o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int t = t0; t < t1; ++t) {
-    const long long kr = chunk_kv_row(a, s.slot, t, 0, head), vr = chunk_kv_row(a, s.slot, t, 1, head);
+    const long long kr = chunk_kv_row(a, slot, t, 0, head), vr = chunk_kv_row(a, slot, t, 1, head);
     const int at = (((lane >> 1) ^ (t & 7)) << 3) + (lane & 1) * 4;
     uint2 kv = {}, vv = {};
     if (kr >= 0) {
@@ -297,10 +322,24 @@ __device__ __noinline__ void chunk_row(const ChunkArgs& a, const ChunkSeq& s, in
   if (l != l) m = l;  // a score that is not a number: what joins this with other ranges must see it
 }
 
+// One block's part in a CTA's range, as the walk hands it on.
+struct ChunkBlock {
+  int more;            // 0: the range is over
+  int row0, ntok;      // its rows of the call
+  int pos0;            // the position of the first of them
+  int head, slot;
+  int t0, nt, tiles;   // key tiles [t0, t0 + nt) of the block's `tiles`
+  int pad;
+  long long base;
+};
+constexpr int CHUNK_BLOCKS = 2;
+
 struct ChunkBars {
-  uint64_t q_full, q_free, q_done;  // q_done: the block's last Q K^T of both groups is over
+  uint64_t q_full, q_free;
   uint64_t kv_full[CHUNK_STAGES], kv_free[CHUNK_STAGES];
-  uint64_t s_full[2], p_full[2], pv_done[2], o_free[2], merge_full;
+  uint64_t s_full[2], p_full[2][2], pv_done[2], o_free[2], merge_full;
+  uint64_t block_full[CHUNK_BLOCKS], block_free[CHUNK_BLOCKS];
+  ChunkBlock block[CHUNK_BLOCKS];
   uint32_t tmem;
   int abort_flag;
   // the range's first block
@@ -308,7 +347,7 @@ struct ChunkBars {
   long long base, total;
   long long scan[CHUNK_THREADS / 32];
 };
-static_assert(sizeof(ChunkBars) <= 512, "ChunkBars sits in the last 512 bytes of the shared memory");
+static_assert(sizeof(ChunkBars) <= 1024, "ChunkBars sits in the last KB of the shared memory");
 
 // ring position of key tile j's K and V in a block of n tiles: K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1)
 __device__ __forceinline__ int chunk_k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
@@ -334,19 +373,23 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 
   if (tid == 0) {
     mbar_init(&B.q_full, 1);
-    mbar_init(&B.q_free, 6);
-    mbar_init(&B.q_done, 2);
+    mbar_init(&B.q_free, 5);
     for (int i = 0; i < CHUNK_STAGES; ++i) {
       mbar_init(&B.kv_full[i], 1);
-      mbar_init(&B.kv_free[i], 2);
+      mbar_init(&B.kv_free[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B.s_full[i], 1);
-      mbar_init(&B.p_full[i], 4);
+      mbar_init(&B.p_full[i][0], 4);
+      mbar_init(&B.p_full[i][1], 4);
       mbar_init(&B.pv_done[i], 1);
       mbar_init(&B.o_free[i], 4);
     }
     mbar_init(&B.merge_full, 4);
+    for (int i = 0; i < CHUNK_BLOCKS; ++i) {
+      mbar_init(&B.block_full[i], 1);
+      mbar_init(&B.block_free[i], 10);
+    }
     B.abort_flag = 0;
     B.any = 0;
     fence_mbar_init();
@@ -355,7 +398,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     tmem_alloc(&B.tmem, 512);
     tmem_relinquish();
   }
-  if (warp == 10 && lane == 0) {
+  if (warp == 9 && lane == 0) {
     tma_prefetch_desc(&q_big);
     tma_prefetch_desc(&q_small);
     tma_prefetch_desc(&kv_map);
@@ -412,19 +455,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   __syncthreads();
   const uint32_t tmem = B.tmem;
   volatile int* abort_flag = &B.abort_flag;
-  ChunkWalk w;
-  bool more = B.any != 0;
-  if (more) {
-    w.i = B.i;
-    w.g = B.g;
-    w.k = B.k;
-    w.base = B.base;
-    w.lo = lo;
-    w.hi = hi;
-    w.s = chunk_seq(a, w.i);
-    w.nb = (w.s.n + bt - 1) / bt;
-    more = chunk_fit(a, w, bt);
-  }
+  // block n of the range: 1 there, 0 the range is over, -1 a wait gave up
+  auto take = [&](uint32_t n) {
+    if (!chunk_wait(&B.block_full[n % CHUNK_BLOCKS], (n / CHUNK_BLOCKS) & 1, abort_flag)) return -1;
+    return B.block[n % CHUNK_BLOCKS].more;
+  };
+  auto give_back = [&](uint32_t n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
+  };
   ChunkMeta* meta = reinterpret_cast<ChunkMeta*>(a.ws + static_cast<size_t>(cta) * 64);
   if (tid == 0) meta->state = 0;
 
@@ -434,14 +473,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     const int grp = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + grp * 128 + lanes, t_o = tmem + 256 + grp * 128 + lanes;
-    uint32_t n_s = 0, n_pv = 0, n_merge = 0, n_unit = 0;  // tiles of this group, merges and blocks so far
-    for (; more; more = chunk_next(a, w, bt), ++n_unit) {
-      const int tok0 = w.k * bt, ntok = min(w.s.n - tok0, bt), nt = w.t1 - w.t0;
-      const bool pair = ntok > T_tok;
-      const int tok = (pair ? grp * T_tok : 0) + row / group;
-      const bool valid = row < T_tok * group && tok < ntok;
-      const int pos = w.s.len - w.s.n + tok0 + tok;  // the row's position
+    uint32_t n_s = 0, n_pv = 0, n_merge = 0;  // tiles of this group and merges so far
+    for (uint32_t n_unit = 0; take(n_unit) == 1; give_back(n_unit), ++n_unit) {
+      const ChunkBlock& d = B.block[n_unit % CHUNK_BLOCKS];
+      const int nt = d.nt;
+      const bool pair = d.ntok > T_tok;
+      const bool valid = row < T_tok * group && (pair ? grp * T_tok : 0) + row / group < d.ntok;
       const bool live = __any_sync(0xffffffffu, valid);
+      // the last key that the row sees, counted from the range's first
+      const int limit = valid ? d.pos0 + (pair ? grp * T_tok : 0) + row / group - d.t0 * CHUNK_KT : -1;
       const int step = pair ? 1 : 2, first = pair ? 0 : grp;
       float m = -INFINITY, l = 0.0f;
       for (int j = first; j < nt; j += step) {
@@ -459,20 +499,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
             for (int c = 0; c < 128; ++c) s[c] = -s[c];
           }
-          const int limit = valid ? pos - (w.t0 + j) * CHUNK_KT : -1;  // last key of the tile that the row sees
-          if (__any_sync(0xffffffffu, limit < CHUNK_KT - 1)) {
+          const int last = limit - j * CHUNK_KT;  // in this tile
+          if (__any_sync(0xffffffffu, last < CHUNK_KT - 1)) {
 #pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] = c <= limit ? s[c] : -INFINITY;
+            for (int c = 0; c < 128; ++c) s[c] = c <= last ? s[c] : -INFINITY;
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+          float mx[4];
 #pragma unroll
-          for (int c = 4; c < 128; c += 4) {
-            mx[0] = fmaxf(mx[0], s[c]);
-            mx[1] = fmaxf(mx[1], s[c + 1]);
-            mx[2] = fmaxf(mx[2], s[c + 2]);
-            mx[3] = fmaxf(mx[3], s[c + 3]);
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          for (int c = 0; c < 4; ++c) mx[c] = max3(s[c], s[c + 4], s[c + 8]);
+#pragma unroll
+          for (int c = 12; c < 124; c += 8)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[c + x], s[c + x + 4]);
+          const float top =
+              fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], fmaxf(s[124], s[125]), fmaxf(s[126], s[127]))) * a.scale_log2;
           const bool raise = top > m + CHUNK_RESCALE;
           if (j == first) {
             m = top;
@@ -495,31 +535,39 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             if (raise) m = top;
           }
           const float base = m == -INFINITY ? 0.0f : m;
-          float sum[4] = {};
+          const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), base2 = pack2(-base, -base);
+          uint64_t sum[2] = {0, 0};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t p[32];
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {
+            for (int c = 0; c < 32; ++c) {
               const int x = h * 64 + c * 2;
-              const float p0 = ex2(fmaf(s[x], a.scale_log2, -base)), p1 = ex2(fmaf(s[x + 1], a.scale_log2, -base));
-              const float p2 = ex2(fmaf(s[x + 2], a.scale_log2, -base)), p3 = ex2(fmaf(s[x + 3], a.scale_log2, -base));
-              sum[0] += p0;
-              sum[1] += p1;
-              sum[2] += p2;
-              sum[3] += p3;
+              float e0, e1;
+              unpack2(fma2(pack2(s[x], s[x + 1]), scale2, base2), e0, e1);
+              const float p0 = ex2(e0), p1 = ex2(e1);
+              sum[c & 1] = add2(sum[c & 1], pack2(p0, p1));
               p[c] = TT::from_f32(p0, p1);
-              p[c + 1] = TT::from_f32(p2, p3);
             }
             tmem_st_x32(t_s + h * 32, p);
+            if (h == 0) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&B.p_full[grp][0]);
+            }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float s0, s1;
+          unpack2(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
           tmem_wait_st();
+        } else if (lane == 0) {
+          mbar_arrive(&B.p_full[grp][0]);
         }
         ++n_pv;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B.p_full[grp]);
+        if (lane == 0) mbar_arrive(&B.p_full[grp][1]);
       }
       if (l != l) m = l;  // a score that is not a number must show in every join
       // ---- the block's end
@@ -531,8 +579,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const bool merge = !pair && nt > 1;
       if (grp == 1 && !pair) {
         if (had) {
-          // O goes where Q was: the other group's products may still read it
-          if (!chunk_wait(&B.q_done, n_unit & 1, abort_flag)) goto softmax_out;
+          // (O goes where Q was: this group's last P V was issued after the block's last Q K^T)
           if (live) {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -571,11 +618,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           else m = top;
         }
       }
-      const bool whole = w.t0 == 0 && w.t1 == w.nt;
+      const bool whole = nt == d.tiles;
+      const int tok = (pair ? grp * T_tok : 0) + row / group, pos = d.pos0 + tok;
       const bool seen = pos >= 0;
-      const int out_row = w.s.row0 + tok0 + tok, qhead = w.g * group + row % group;
+      const int out_row = d.row0 + tok, qhead = d.head * group + row % group;
       const int prow = (pair ? grp * 128 : 0) + row;
-      float* part = chunk_part(a, grid, w.t0 == 0 ? 2 * cta + 1 : 2 * cta);
+      float* part = chunk_part(a, grid, d.t0 == 0 ? 2 * cta + 1 : 2 * cta);
       float bad = 0.0f;
       if (live) {
         const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
@@ -627,7 +675,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const int r_pos = __shfl_sync(0xffffffffu, pos, src), r_prow = __shfl_sync(0xffffffffu, prow, src);
         float rm, rl;
         float4 o;
-        chunk_row<BF16>(a, w.s, r_row, r_head, w.t0 * CHUNK_KT, min(w.t1 * CHUNK_KT, r_pos + 1), rm, rl, o);
+        chunk_row<BF16>(a, d.slot, r_row, r_head, d.t0 * CHUNK_KT, min((d.t0 + nt) * CHUNK_KT, r_pos + 1), rm, rl, o);
         if (whole) {
           const float inv = 1.0f / rl;
           uint2 v;
@@ -646,118 +694,134 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
         }
       }
-      if (!whole && w.t0 == 0 && tid == 0) {
-        meta->row0 = w.s.row0 + tok0;
-        meta->ntok = ntok;
-        meta->head = w.g;
-        meta->nt = w.nt;
-        meta->pos0 = w.s.len - w.s.n + tok0;
-        meta->base = w.base;
+      if (!whole && d.t0 == 0 && tid == 0) {
+        meta->row0 = d.row0;
+        meta->ntok = d.ntok;
+        meta->head = d.head;
+        meta->nt = d.tiles;
+        meta->pos0 = d.pos0;
+        meta->base = d.base;
         meta->total = total;
         meta->state = 1;
       }
     }
   softmax_out:;
-  } else if (warp < 10) {
+  } else if (warp == 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ================================================================ MMA issue
-    const int grp = warp - 8;
-    const uint32_t t_s = tmem + grp * 128, t_o = tmem + 256 + grp * 128;
     constexpr uint32_t id_qk = chunk_idesc<BF16>(false), id_pv = chunk_idesc<BF16>(true);
-    uint32_t n_unit = 0, n_tile = 0, n_out = 0, ring = 0;
-    // Both issuers wait for every ring position, in order, and both release it: by the MMAs that read it, or, for a
-    // stage of a one-tile block that only the other group reads, at once.  So neither can miss a phase.
-    uint32_t landed = 0;
-    auto ready = [&](uint32_t upto, bool pass) {
-      for (; landed < upto; ++landed) {
-        const uint32_t st = landed % CHUNK_STAGES;
-        if (!chunk_wait(&B.kv_full[st], (landed / CHUNK_STAGES) & 1, abort_flag)) return false;
-        if (pass && lane == 0) mbar_arrive(&B.kv_free[st]);
+    uint32_t n_tile[2] = {0, 0}, n_out[2] = {0, 0}, ring = 0;
+    // S of group g = Q K^T with the key tile at ring position `it`
+    auto scores = [&](int g, uint32_t it, bool pair) {
+      if (lane == 0) {
+        const uint64_t dq = smem_desc_sw128(smem_u32(sm_q) + (pair ? g * CHUNK_STAGE_BYTES : 0));
+        const uint64_t dk = smem_desc_sw128(smem_u32(sm_kv + (it % CHUNK_STAGES) * CHUNK_STAGE_BYTES));
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const uint32_t off = ((x >> 2) * CHUNK_HALF_BYTES + (x & 3) * 32) >> 4;
+          umma_f16_ss(tmem + g * 128, dq + off, dk + off, id_qk, x > 0 ? 1u : 0u);
+        }
+        umma_commit(&B.s_full[g]);
       }
+      __syncwarp();
+    };
+    // O of group g += P V, P by halves as the softmax group hands them over
+    auto values = [&](int g, uint32_t it, bool first) {
+      if (first) {  // the block before has been read out
+        if (n_out[g] && !chunk_wait(&B.o_free[g], (n_out[g] - 1) & 1, abort_flag)) return false;
+        ++n_out[g];
+      }
+      const uint64_t dv = smem_desc_v(smem_u32(sm_kv + (it % CHUNK_STAGES) * CHUNK_STAGE_BYTES));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!chunk_wait(&B.p_full[g][h], n_tile[g] & 1, abort_flag)) return false;
+        tc_fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int x = h * 4; x < h * 4 + 4; ++x)
+            umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + x * 8, dv + x * (2048 >> 4), id_pv, (!first || x > 0) ? 1u : 0u);
+          if (h == 1) umma_commit(&B.pv_done[g]);
+        }
+        __syncwarp();
+      }
+      ++n_tile[g];
       return true;
     };
-    auto mine = [&](uint32_t it, bool pair) { return ready(it, !pair) && ready(it + 1, false); };
-    for (; more; more = chunk_next(a, w, bt)) {
-      const int tok0 = w.k * bt, ntok = min(w.s.n - tok0, bt), nt = w.t1 - w.t0;
-      const bool pair = ntok > T_tok;
-      const int step = pair ? 1 : 2, first = pair ? 0 : grp;
-      const int end = w.s.len - w.s.n + tok0 + ntok;  // positions the block sees
-      const uint32_t q_addr = smem_u32(sm_q) + (pair ? grp * CHUNK_STAGE_BYTES : 0);
+    auto release = [&](uint32_t it) {
+      if (lane == 0) umma_commit(&B.kv_free[it % CHUNK_STAGES]);
+      __syncwarp();
+    };
+    auto landed = [&](uint32_t it) {
+      return chunk_wait(&B.kv_full[it % CHUNK_STAGES], (it / CHUNK_STAGES) & 1, abort_flag);
+    };
+    for (uint32_t n_unit = 0; take(n_unit) == 1; ++n_unit) {
+      const ChunkBlock& d = B.block[n_unit % CHUNK_BLOCKS];
+      const int nt = d.nt, t0 = d.t0;
+      const bool pair = d.ntok > T_tok;
+      const int end = d.pos0 + d.ntok;  // positions the block sees
+      give_back(n_unit);
       if (!chunk_wait(&B.q_full, n_unit & 1, abort_flag)) goto mma_out;
-      if (first >= nt) {  // a one-tile block of one key tile: nothing for the second group
-        if (lane == 0) {
-          mbar_arrive(&B.q_free);
-          mbar_arrive(&B.q_done);
-        }
+      // a pair's groups share the key tiles; those of a one-tile block take them in turn
+      if (!landed(ring)) goto mma_out;
+      scores(0, ring, pair);
+      if (pair) {
+        scores(1, ring, pair);
+        release(ring);
       } else {
-        for (int j = first - step; j < nt; j += step) {
-          if (j >= 0) {
-            const uint32_t it = ring + chunk_v_at(j, nt), st = it % CHUNK_STAGES;
-            if (!mine(it, pair)) goto mma_out;
-            uint8_t* v = sm_kv + st * CHUNK_STAGE_BYTES;
-            const int held = end - (w.t0 + j) * CHUNK_KT;  // positions of this tile that the block sees
-            if (held < CHUNK_KT) {
-              // both issuers may clear the same rows: the same zeros
-              for (int x = max(held, 0) * 8 + lane; x < CHUNK_KT * 8; x += 32) {
-                reinterpret_cast<uint4*>(v)[x] = make_uint4(0, 0, 0, 0);
-                reinterpret_cast<uint4*>(v + CHUNK_HALF_BYTES)[x] = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-            }
-            if (j == first) {
-              if (n_out && !chunk_wait(&B.o_free[grp], (n_out - 1) & 1, abort_flag)) goto mma_out;
-              ++n_out;
-            }
-            if (!chunk_wait(&B.p_full[grp], n_tile & 1, abort_flag)) goto mma_out;
-            ++n_tile;
-            tc_fence_after();
-            if (lane == 0) {
-              const uint64_t d = smem_desc_v(smem_u32(v));
-#pragma unroll
-              for (int x = 0; x < 8; ++x)
-                umma_f16_ts(t_o, t_s + x * 8, d + x * (2048 >> 4), id_pv, (j > first || x > 0) ? 1u : 0u);
-              umma_commit(&B.pv_done[grp]);
-              umma_commit(&B.kv_free[st]);
-            }
-            __syncwarp();
-          }
-          const int jn = j + step;
-          if (jn < nt) {
-            const uint32_t it = ring + chunk_k_at(jn), st = it % CHUNK_STAGES;
-            if (!mine(it, pair)) goto mma_out;
-            tc_fence_after();
-            if (lane == 0) {
-              const uint64_t dq = smem_desc_sw128(q_addr), dk = smem_desc_sw128(smem_u32(sm_kv + st * CHUNK_STAGE_BYTES));
-#pragma unroll
-              for (int x = 0; x < 8; ++x) {
-                const uint32_t off = ((x >> 2) * CHUNK_HALF_BYTES + (x & 3) * 32) >> 4;
-                umma_f16_ss(t_s, dq + off, dk + off, id_qk, x > 0 ? 1u : 0u);
-              }
-              umma_commit(&B.s_full[grp]);
-              umma_commit(&B.kv_free[st]);
-              if (jn + step >= nt) {
-                umma_commit(&B.q_free);
-                umma_commit(&B.q_done);
-              }
-            }
-            __syncwarp();
-          }
+        release(ring);
+        if (nt > 1) {
+          if (!landed(ring + 1)) goto mma_out;
+          scores(1, ring + 1, pair);
+          release(ring + 1);
         }
       }
-      ++n_unit;
+      if (nt <= (pair ? 1 : 2) && lane == 0) umma_commit(&B.q_free);
+      for (int j = 0; j < nt; ++j) {
+        // ring order: K0 K1 V0 K2 V1 K3 ...
+        const int jn = j + (pair ? 1 : 2);
+        const uint32_t iv = ring + chunk_v_at(j, nt), ik = ring + chunk_k_at(jn);
+        if (pair && jn < nt && !landed(ik)) goto mma_out;
+        if (!landed(iv)) goto mma_out;
+        const int held = end - (t0 + j) * CHUNK_KT;  // positions of this tile that the block sees
+        if (held < CHUNK_KT) {
+          uint8_t* v = sm_kv + (iv % CHUNK_STAGES) * CHUNK_STAGE_BYTES;
+          for (int x = max(held, 0) * 8 + lane; x < CHUNK_KT * 8; x += 32) {
+            reinterpret_cast<uint4*>(v)[x] = make_uint4(0, 0, 0, 0);
+            reinterpret_cast<uint4*>(v + CHUNK_HALF_BYTES)[x] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const int g = pair ? 0 : j & 1;
+        if (!values(g, iv, j < (pair ? 1 : 2))) goto mma_out;
+        if (!pair) {
+          release(iv);
+          if (jn < nt && !landed(ik)) goto mma_out;
+        }
+        if (jn < nt) scores(g, ik, pair);
+        if (pair) {
+          if (!values(1, iv, j == 0)) goto mma_out;
+          release(iv);
+          if (jn < nt) scores(1, ik, pair);
+        }
+        if (jn < nt) {
+          release(ik);
+          if (jn == nt - 1 && lane == 0) umma_commit(&B.q_free);
+        }
+      }
       ring += 2 * nt;
-      if (!ready(ring, !pair)) goto mma_out;
     }
   mma_out:;
-  } else if (warp == 10) {
+  } else if (warp == 9) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ================================================================ copies
-    uint32_t n_unit = 0, ring = 0;
-    for (; more; more = chunk_next(a, w, bt)) {
-      const int tok0 = w.k * bt, ntok = min(w.s.n - tok0, bt), nt = w.t1 - w.t0;
+    uint32_t ring = 0;
+    for (uint32_t n_unit = 0; take(n_unit) == 1; ++n_unit) {
+      const ChunkBlock& d = B.block[n_unit % CHUNK_BLOCKS];
+      const int ntok = d.ntok, nt = d.nt, t0 = d.t0, row0 = d.row0, head = d.head, slot = d.slot;
       const bool pair = ntok > T_tok;
-      const int end = w.s.len - w.s.n + tok0 + ntok;
+      const int end = d.pos0 + ntok;
+      give_back(n_unit);
       if (n_unit && !chunk_wait(&B.q_free, (n_unit - 1) & 1, abort_flag)) goto copy_out;
       if (lane == 0) {
         const bool small = ntok <= 8;
@@ -766,19 +830,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         for (int x = 0; x < tiles; ++x)
           for (int h = 0; h < 2; ++h)
             tma_load_4d(sm_q + x * CHUNK_STAGE_BYTES + h * CHUNK_HALF_BYTES, small ? &q_small : &q_big, &B.q_full, 0,
-                        w.g * group, w.s.row0 + tok0 + x * T_tok, h);
+                        head * group, row0 + x * T_tok, h);
       }
       __syncwarp();
-      const int pages = min((max(end, 0) + CHUNK_PAGE - 1) / CHUNK_PAGE, 2 * w.t1);  // of the range, from page 0 on
+      const int pages = min((max(end, 0) + CHUNK_PAGE - 1) / CHUNK_PAGE, 2 * (t0 + nt));  // of the range, from page 0 on
       int page_of = 0, from = -1;
       for (int x = 0; x < 2 * nt; ++x) {
         // ring order: K0 K1 V0 K2 V1 ...
         const bool is_v = nt == 1 ? x == 1 : x == 2 * nt - 1 || (x > 1 && (x & 1) == 0);
         const int j = x == 2 * nt - 1 ? nt - 1 : is_v ? (x - 2) / 2 : (x + 1) / 2;
-        const int p0 = 2 * (w.t0 + j), have = min(2, pages - p0);
+        const int p0 = 2 * (t0 + j), have = min(2, pages - p0);
         if (from < 0 || p0 < from || p0 + 2 > from + 32) {  // page ids, 32 at a time
           from = is_v ? p0 : max(p0 - 4, 0);
-          page_of = from + lane < pages ? a.page_table[static_cast<size_t>(w.s.slot) * a.max_pages + from + lane] : -1;
+          page_of = from + lane < pages ? a.page_table[static_cast<size_t>(slot) * a.max_pages + from + lane] : -1;
         }
         const uint32_t it = ring + x, st = it % CHUNK_STAGES;
         if (it >= CHUNK_STAGES && !chunk_wait(&B.kv_free[st], (it / CHUNK_STAGES - 1) & 1, abort_flag)) goto copy_out;
@@ -792,14 +856,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             // a page outside the pool reads as zeros: rows behind the map's last
             const int r = page < 0 || page >= a.pool_pages
                               ? a.pool_pages * a.layers * 2 * a.nkv * CHUNK_PAGE
-                              : (((page * a.layers + a.layer) * 2 + (is_v ? 1 : 0)) * a.nkv + w.g) * CHUNK_PAGE;
+                              : (((page * a.layers + a.layer) * 2 + (is_v ? 1 : 0)) * a.nkv + head) * CHUNK_PAGE;
             for (int h = 0; h < 2; ++h)
               tma_load_3d(dst + h * CHUNK_HALF_BYTES + y * (CHUNK_PAGE * 128), &kv_map, &B.kv_full[st], 0, r, h);
           }
         }
         __syncwarp();
       }
-      ++n_unit;
       ring += 2 * nt;
     }
   copy_out:
@@ -814,8 +877,47 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         while (!mbar_try_wait(&B.q_full, x) && globaltimer() - t0 < 40000000ull) {
         }
     }
-  } else {
+  } else if (warp == 11) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  } else {
+    // ================================================================ the walk
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    ChunkWalk w;
+    bool more = B.any != 0;
+    if (more) {
+      w.i = B.i;
+      w.g = B.g;
+      w.k = B.k;
+      w.base = B.base;
+      w.lo = lo;
+      w.hi = hi;
+      w.s = chunk_seq(a, w.i);
+      w.nb = (w.s.n + bt - 1) / bt;
+      more = chunk_fit(a, w, bt);
+    }
+    for (uint32_t n = 0;; ++n) {
+      if (n >= CHUNK_BLOCKS && !chunk_wait(&B.block_free[n % CHUNK_BLOCKS], (n / CHUNK_BLOCKS - 1) & 1, abort_flag)) break;
+      if (lane == 0) {
+        ChunkBlock& d = B.block[n % CHUNK_BLOCKS];
+        d.more = more;
+        if (more) {
+          const int tok0 = w.k * bt;
+          d.row0 = w.s.row0 + tok0;
+          d.ntok = min(w.s.n - tok0, bt);
+          d.pos0 = w.s.len - w.s.n + tok0;
+          d.head = w.g;
+          d.slot = w.s.slot;
+          d.t0 = w.t0;
+          d.nt = w.t1 - w.t0;
+          d.tiles = w.nt;
+          d.base = w.base;
+        }
+        mbar_arrive(&B.block_full[n % CHUNK_BLOCKS]);
+      }
+      __syncwarp();
+      if (!more) break;
+      more = chunk_next(a, w, bt);
+    }
   }
   tc_fence_before();
   __syncthreads();
