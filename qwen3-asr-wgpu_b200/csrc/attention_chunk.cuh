@@ -262,6 +262,14 @@ __host__ __device__ constexpr uint32_t chunk_idesc(bool b_mn_major) {
   return umma_idesc_f16_m128(128) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u);
 }
 
+// One lane of a converged warp, the same one each time.  (Behind this the compiler issues MMAs from uniform registers; behind
+// `lane == 0` it does not, and an MMA takes 85 cycles next to busy warps instead of 69.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // A bounded wait of a whole warp: every lane sees the phase complete, or all of them give up together.
 __device__ __forceinline__ bool chunk_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
@@ -713,7 +721,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint32_t n_tile[2] = {0, 0}, n_out[2] = {0, 0}, ring = 0;
     // S of group g = Q K^T with the key tile at ring position `it`
     auto scores = [&](int g, uint32_t it, bool pair) {
-      if (lane == 0) {
+      if (elect_one()) {
         const uint64_t dq = smem_desc_sw128(smem_u32(sm_q) + (pair ? g * CHUNK_STAGE_BYTES : 0));
         const uint64_t dk = smem_desc_sw128(smem_u32(sm_kv + (it % CHUNK_STAGES) * CHUNK_STAGE_BYTES));
 #pragma unroll
@@ -736,7 +744,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       for (int h = 0; h < 2; ++h) {
         if (!chunk_wait(&B.p_full[g][h], n_tile[g] & 1, abort_flag)) return false;
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
 #pragma unroll
           for (int x = h * 4; x < h * 4 + 4; ++x)
             umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + x * 8, dv + x * (2048 >> 4), id_pv, (!first || x > 0) ? 1u : 0u);
@@ -748,7 +756,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       return true;
     };
     auto release = [&](uint32_t it) {
-      if (lane == 0) umma_commit(&B.kv_free[it % CHUNK_STAGES]);
+      if (elect_one()) umma_commit(&B.kv_free[it % CHUNK_STAGES]);
       __syncwarp();
     };
     auto landed = [&](uint32_t it) {
@@ -775,7 +783,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           release(ring + 1);
         }
       }
-      if (nt <= (pair ? 1 : 2) && lane == 0) umma_commit(&B.q_free);
+      if (nt <= (pair ? 1 : 2) && elect_one()) umma_commit(&B.q_free);
       for (int j = 0; j < nt; ++j) {
         // ring order: K0 K1 V0 K2 V1 K3 ...
         const int jn = j + (pair ? 1 : 2);
@@ -806,7 +814,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         if (jn < nt) {
           release(ik);
-          if (jn == nt - 1 && lane == 0) umma_commit(&B.q_free);
+          if (jn == nt - 1 && elect_one()) umma_commit(&B.q_free);
         }
       }
       ring += 2 * nt;
