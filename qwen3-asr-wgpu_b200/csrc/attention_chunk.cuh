@@ -7,23 +7,26 @@
 //
 // The products are tcgen05 MMAs of 128 rows.  A kv head's nq / nkv = G query heads share its keys, so
 // the rows of a tile are packed: row r is token r / G, head r % G of the group (T tokens a tile, T the
-// largest multiple of 8 with T * G <= 128).  A block is two row tiles; per tile of 128 keys
+// largest multiple of 8 with T * G <= 128).  A block is two row tiles; per page of 64 keys
 //   S = Q K^T        A: Q in shared memory, B: K in shared memory (positions x dims, K-major)
 //   P = 2^(S - m)    one thread per row, straight from and back to tensor memory, where P takes S's place
 //   O += P V         A: P in tensor memory, B: V in shared memory (MN-major), O in tensor memory
 // A page's swizzle (chunk c of position p at c ^ (p % 8)) is, for each 64-dim half of its rows, the
 // tensor core's own 128-byte swizzle, so pages are copied by TMA as they are and used as operands.
+// Tensor memory holds two S tiles and O of each row tile: while a tile's softmax runs, the next tile's
+// product is under way, so the softmax never waits for it.  (Two S tiles of 128 keys would not fit beside O; of 64 keys
+// Q K^T runs at 3/4 of the tensor cores' rate, its operands coming from shared memory, which costs less than the
+// wait: one S tile of 128 keys ran at 4050 cycles per 128 keys and two row tiles, half of them waiting.)
 // P is rounded to the cache's type for the second product, as the tensor core wants it; the sum of P
 // is taken before that rounding.  m is raised, and O rescaled, only when a row's maximum has grown by more than
 // 2^8 (P then stays below 2^8, far inside f16), so the rescaling, a round trip over O, is rare.
 //
-// Roles: warps 0-3 and 4-7 are two softmax groups, one per row tile; warp 8 issues the MMAs, the groups' in turn, so
-// that one group's products run under the other's softmax (two issuers, one a group, fall into step: both
-// groups then wait together); warp 9 copies Q and the pages into a ring of 128-position stages; warp 10
-// walks the schedule and hands the others one block after the other through shared memory, which keeps the walk out of
-// their registers.  The second product starts on the first half of P while the second half is computed.  A block of one
-// row tile only (a decode step, a short chunk) gives its even key tiles to the first group and the odd ones to the
-// second, which then merge, so both always have work.
+// Roles: three threads, one a warp, steer: warp 0's issues Q K^T, warp 1's P V, each with its own ring of pages, so neither's
+// waits hold up the other; warp 2's copies Q and the pages.  Warp 3 walks the schedule and hands the others one block
+// after the other through shared memory, which keeps the walk out of their registers, and clears V rows for
+// warp 1.  Warps 4-7 and 8-11 are two softmax groups, one per row tile.  A block of one row tile only (a
+// decode step, a short chunk) gives its even key tiles to the first group and the odd ones to the second; the first
+// then joins both results, which stand in the same tensor memory lanes.  So both always have work.
 //
 // Work split: every (request, kv head, block) costs its key tiles plus CHUNK_BLOCK_COST; the costs of the whole call,
 // laid end to end, are cut into one equal range per CTA.  A block that a cut goes through leaves f32
@@ -64,16 +67,18 @@ struct ChunkArgs {
 };
 
 constexpr int CHUNK_THREADS = 384;
-constexpr int CHUNK_KT = 128;                     // keys per tile
-constexpr int CHUNK_STAGES = 5;
+constexpr int CHUNK_KT = CHUNK_PAGE;              // keys per tile
+constexpr int CHUNK_STAGES = 4;                   // of K and of V each
 constexpr int CHUNK_STAGE_BYTES = CHUNK_KT * CHUNK_DIM * 2;
-constexpr int CHUNK_HALF_BYTES = CHUNK_KT * 128;  // 128 rows of one 64-dim half
-constexpr int CHUNK_Q_BYTES = 2 * CHUNK_STAGE_BYTES;
-constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + CHUNK_STAGES * CHUNK_STAGE_BYTES + 2048;
-constexpr int CHUNK_BLOCK_COST = 1;               // a block's Q copy, first and last steps, in key tiles
-constexpr int CHUNK_SNAP = 1;                     // a cut this near to a block's edge moves onto it
+constexpr int CHUNK_HALF_BYTES = CHUNK_KT * 128;  // the rows' first or second 64 dims
+constexpr int CHUNK_Q_TILE = 128 * CHUNK_DIM * 2, CHUNK_Q_HALF = CHUNK_Q_TILE / 2;
+constexpr int CHUNK_Q_BYTES = 2 * CHUNK_Q_TILE;
+constexpr int CHUNK_OUT_BYTES = 32 * 128;          // per softmax warp: half of its rows' output
+constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + 2 * CHUNK_STAGES * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 2048;
+constexpr int CHUNK_BLOCK_COST = 2;               // a block's Q copy, first and last steps, in key tiles
+constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
-constexpr uint64_t CHUNK_WAIT_NS = 10 * QASR_WAIT_NS;  // rows computed again by chunk_row keep the others waiting
+constexpr uint32_t CHUNK_WAIT_STEPS = (10 * QASR_WAIT_NS) >> 20;  // rows computed again by chunk_row keep the others waiting
 constexpr int CHUNK_PART_ROWS = 256;
 constexpr int CHUNK_PART_FLOATS = (CHUNK_DIM + 2) * CHUNK_PART_ROWS;  // [o 0..127, m, l][row]
 
@@ -258,8 +263,8 @@ __device__ __forceinline__ uint64_t smem_desc_v(uint32_t smem_addr) {
          (static_cast<uint64_t>(2u) << 61);
 }
 template <bool BF16>
-__host__ __device__ constexpr uint32_t chunk_idesc(bool b_mn_major) {
-  return umma_idesc_f16_m128(128) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u);
+__host__ __device__ constexpr uint32_t chunk_idesc(uint32_t n, bool b_mn_major) {
+  return umma_idesc_f16_m128(n) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u);
 }
 
 // One lane of a converged warp, the same one each time.  (Behind this the compiler issues MMAs from uniform registers; behind
@@ -271,22 +276,37 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // A bounded wait of a whole warp: every lane sees the phase complete, or all of them give up together.
+// (The clock is a slow read: it is looked at only once a good number of tries, each of which may itself be suspended
+// for a while, has gone by.)
 __device__ __forceinline__ bool chunk_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  const uint64_t t0 = globaltimer();
-  while (true) {
+  uint32_t t0 = 0;  // the clock's bits 20 and up (steps of about a millisecond)
+  for (uint32_t n = 1;; ++n) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    int quit = 0;
-    if ((threadIdx.x & 31) == 0) {
-      if (*abort_flag) {
-        quit = 1;
-      } else if (globaltimer() - t0 > CHUNK_WAIT_NS) {
-        *abort_flag = 1;
-        quit = 1;
+    if ((n & 63) == 0) {
+      const uint32_t now = static_cast<uint32_t>(globaltimer() >> 20);
+      if (n == 64) t0 = now;
+      int quit = 0;
+      if ((threadIdx.x & 31) == 0) {
+        if (now - t0 > CHUNK_WAIT_STEPS) *abort_flag = 1;
+        quit = *abort_flag;
       }
+      if (__shfl_sync(0xffffffffu, quit, 0)) return false;
     }
-    if (__shfl_sync(0xffffffffu, quit, 0)) return false;
   }
+}
+
+// The same for one thread.
+__device__ __forceinline__ bool chunk_wait_one(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  uint32_t t0 = 0;
+  for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n) {
+    if ((n & 63) == 0) {
+      const uint32_t now = static_cast<uint32_t>(globaltimer() >> 20);
+      if (n == 64) t0 = now;
+      if (now - t0 > CHUNK_WAIT_STEPS) *abort_flag = 1;
+      if (*abort_flag) return false;
+    }
+  }
+  return true;
 }
 
 // One row's (m, l, o) over the positions [t0, t1) without matrix instructions: a warp, lane l holding the dims
@@ -337,15 +357,19 @@ struct ChunkBlock {
   int pos0;            // the position of the first of them
   int head, slot;
   int t0, nt, tiles;   // key tiles [t0, t0 + nt) of the block's `tiles`
-  int pad;
+  int nt0;             // of two row tiles: how many of the nt the first one sees
   long long base;
+  int pages[16];       // the first pages of the range
 };
-constexpr int CHUNK_BLOCKS = 2;
+constexpr int CHUNK_BLOCKS = 3;
 
 struct ChunkBars {
-  uint64_t q_full, q_free;
-  uint64_t kv_full[CHUNK_STAGES], kv_free[CHUNK_STAGES];
-  uint64_t s_full[2], p_full[2][2], pv_done[2], o_free[2], merge_full;
+  uint64_t q_full[2], q_free[2];               // of a row tile's place
+  uint64_t kv_full[2][CHUNK_STAGES], kv_free[2][CHUNK_STAGES];  // K, V
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_done[2], o_free[2], merge_full;
+  uint64_t clear_ask, clear_done;              // rows of a V stage to be zeroed
+  uint8_t* clear_at;
+  int clear_from;
   uint64_t block_full[CHUNK_BLOCKS], block_free[CHUNK_BLOCKS];
   ChunkBlock block[CHUNK_BLOCKS];
   uint32_t tmem;
@@ -357,10 +381,6 @@ struct ChunkBars {
 };
 static_assert(sizeof(ChunkBars) <= 1024, "ChunkBars sits in the last KB of the shared memory");
 
-// ring position of key tile j's K and V in a block of n tiles: K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1)
-__device__ __forceinline__ int chunk_k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
-__device__ __forceinline__ int chunk_v_at(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
-
 template <bool BF16>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     attention_chunk_kernel(const __grid_constant__ CUtensorMap q_big, const __grid_constant__ CUtensorMap q_small,
@@ -370,43 +390,50 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t chunk_dsmem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(chunk_dsmem) + 1023) & ~uintptr_t(1023));
   uint8_t* sm_q = smem;                                    // two row tiles, each [2 halves][128 rows][128 B]
-  uint8_t* sm_kv = smem + CHUNK_Q_BYTES;                   // stages of [2 halves][128 positions][128 B]
-  float* sm_ml = reinterpret_cast<float*>(sm_kv + CHUNK_STAGES * CHUNK_STAGE_BYTES);  // [2][128]: group 1's m and l
+  uint8_t* sm_kv = smem + CHUNK_Q_BYTES;                   // stages of K, then of V: [2 halves][64 positions][128 B]
+  uint8_t* sm_out = sm_kv + 2 * CHUNK_STAGES * CHUNK_STAGE_BYTES;  // per softmax warp [32 rows][128 B], chunks of 16 B swizzled
+  float* sm_ml = reinterpret_cast<float*>(sm_out + 8 * CHUNK_OUT_BYTES);  // [2][128]: group 1's m and l
   ChunkBars& B = *reinterpret_cast<ChunkBars*>(reinterpret_cast<uint8_t*>(sm_ml) + 1024);
-  float* sm_o = reinterpret_cast<float*>(sm_q);            // [128 dims][128 rows]: group 1's O of a one-tile block
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grid = gridDim.x, cta = blockIdx.x;
   const int group = a.nq / a.nkv, T_tok = chunk_tile_tokens(group), bt = 2 * T_tok;
 
   if (tid == 0) {
-    mbar_init(&B.q_full, 1);
-    mbar_init(&B.q_free, 5);
+    mbar_init(&B.clear_ask, 1);
+    mbar_init(&B.clear_done, 1);
     for (int i = 0; i < CHUNK_STAGES; ++i) {
-      mbar_init(&B.kv_full[i], 1);
-      mbar_init(&B.kv_free[i], 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&B.kv_full[x][i], 1);
+        mbar_init(&B.kv_free[x][i], 1);
+      }
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&B.s_full[i], 1);
+      mbar_init(&B.s_full[i][0], 1);
+      mbar_init(&B.s_full[i][1], 1);
+      mbar_init(&B.o_done[i], 1);
+      mbar_init(&B.q_full[i], 1);
+      mbar_init(&B.q_free[i], 1);
       mbar_init(&B.p_full[i][0], 4);
       mbar_init(&B.p_full[i][1], 4);
-      mbar_init(&B.pv_done[i], 1);
+      mbar_init(&B.pv_done[i][0], 1);
+      mbar_init(&B.pv_done[i][1], 1);
       mbar_init(&B.o_free[i], 4);
     }
     mbar_init(&B.merge_full, 4);
     for (int i = 0; i < CHUNK_BLOCKS; ++i) {
       mbar_init(&B.block_full[i], 1);
-      mbar_init(&B.block_free[i], 10);
+      mbar_init(&B.block_free[i], 11);
     }
     B.abort_flag = 0;
     B.any = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 0) {
     tmem_alloc(&B.tmem, 512);
     tmem_relinquish();
   }
-  if (warp == 9 && lane == 0) {
+  if (warp == 2 && lane == 0) {
     tma_prefetch_desc(&q_big);
     tma_prefetch_desc(&q_small);
     tma_prefetch_desc(&kv_map);
@@ -472,16 +499,22 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     __syncwarp();
     if (lane == 0) mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
   };
+  // the same for the threads that steer
+  auto wait_one = [&](uint64_t* bar, uint32_t parity) { return chunk_wait_one(bar, parity, abort_flag); };
+  auto take_one = [&](uint32_t n) {
+    if (!wait_one(&B.block_full[n % CHUNK_BLOCKS], (n / CHUNK_BLOCKS) & 1)) return -1;
+    return B.block[n % CHUNK_BLOCKS].more;
+  };
   ChunkMeta* meta = reinterpret_cast<ChunkMeta*>(a.ws + static_cast<size_t>(cta) * 64);
-  if (tid == 0) meta->state = 0;
+  if (tid == 128) meta->state = 0;  // (the thread that may set it to 1)
 
-  if (warp < 8) {
+  if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");  // 256 x 208 + 128 x 88 = the launch's 384 x 168
     // ================================================================ softmax and output
-    const int grp = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int grp = (warp >> 2) - 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + grp * 128 + lanes, t_o = tmem + 256 + grp * 128 + lanes;
-    uint32_t n_s = 0, n_pv = 0, n_merge = 0;  // tiles of this group and merges so far
+    uint32_t n_tile = 0, n_out = 0, n_merge = 0;  // this group's tiles and blocks, and merges, so far
     for (uint32_t n_unit = 0; take(n_unit) == 1; give_back(n_unit), ++n_unit) {
       const ChunkBlock& d = B.block[n_unit % CHUNK_BLOCKS];
       const int nt = d.nt;
@@ -490,43 +523,41 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const bool live = __any_sync(0xffffffffu, valid);
       // the last key that the row sees, counted from the range's first
       const int limit = valid ? d.pos0 + (pair ? grp * T_tok : 0) + row / group - d.t0 * CHUNK_KT : -1;
-      const int step = pair ? 1 : 2, first = pair ? 0 : grp;
+      const int step = pair ? 1 : 2, first = pair ? 0 : grp, count = pair && grp == 0 ? d.nt0 : nt;
       float m = -INFINITY, l = 0.0f;
-      for (int j = first; j < nt; j += step) {
-        if (!chunk_wait(&B.s_full[grp], n_s & 1, abort_flag)) goto softmax_out;
-        ++n_s;
+      for (int j = first; j < count; j += step, ++n_tile) {
+        const uint32_t t_buf = t_s + (n_tile & 1) * CHUNK_KT;
+        if (!chunk_wait(&B.s_full[grp][n_tile & 1], (n_tile >> 1) & 1, abort_flag)) goto softmax_out;
         tc_fence_after();
-        // (not before this block's first S: only then is the barrier's previous phase over)
-        if (pair && grp == 0 && j == 0 && lane == 0) mbar_arrive(&B.q_free);
         if (live) {
-          float s[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_x32(t_s + c * 32, s + c * 32);
+          float s[CHUNK_KT];
+          tmem_ld_x32(t_buf, s);
+          tmem_ld_x32(t_buf + 32, s + 32);
           tmem_wait_ld();
           if (a.negate) {
 #pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] = -s[c];
+            for (int c = 0; c < CHUNK_KT; ++c) s[c] = -s[c];
           }
           const int last = limit - j * CHUNK_KT;  // in this tile
           if (__any_sync(0xffffffffu, last < CHUNK_KT - 1)) {
 #pragma unroll
-            for (int c = 0; c < 128; ++c) s[c] = c <= last ? s[c] : -INFINITY;
+            for (int c = 0; c < CHUNK_KT; ++c) s[c] = c <= last ? s[c] : -INFINITY;
           }
           float mx[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) mx[c] = max3(s[c], s[c + 4], s[c + 8]);
 #pragma unroll
-          for (int c = 12; c < 124; c += 8)
+          for (int c = 12; c < 60; c += 8)
 #pragma unroll
             for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[c + x], s[c + x + 4]);
           const float top =
-              fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], fmaxf(s[124], s[125]), fmaxf(s[126], s[127]))) * a.scale_log2;
+              fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], fmaxf(s[60], s[61]), fmaxf(s[62], s[63]))) * a.scale_log2;
           const bool raise = top > m + CHUNK_RESCALE;
           if (j == first) {
             m = top;
           } else if (__any_sync(0xffffffffu, raise)) {
             // O holds the sums under the old maximum: bring it under the new one
-            if (!chunk_wait(&B.pv_done[grp], (n_pv - 1) & 1, abort_flag)) goto softmax_out;
+            if (!chunk_wait(&B.pv_done[grp][(n_tile - 1) & 1], ((n_tile - 1) >> 1) & 1, abort_flag)) goto softmax_out;
             tc_fence_after();
             const float f = raise ? ex2(m - top) : 1.0f;
 #pragma unroll 1
@@ -545,68 +576,41 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const float base = m == -INFINITY ? 0.0f : m;
           const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), base2 = pack2(-base, -base);
           uint64_t sum[2] = {0, 0};
+          uint32_t p[32];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t p[32];
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const int x = h * 64 + c * 2;
-              float e0, e1;
-              unpack2(fma2(pack2(s[x], s[x + 1]), scale2, base2), e0, e1);
-              const float p0 = ex2(e0), p1 = ex2(e1);
-              sum[c & 1] = add2(sum[c & 1], pack2(p0, p1));
-              p[c] = TT::from_f32(p0, p1);
-            }
-            tmem_st_x32(t_s + h * 32, p);
-            if (h == 0) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&B.p_full[grp][0]);
-            }
+          for (int c = 0; c < 32; ++c) {
+            float e0, e1;
+            unpack2(fma2(pack2(s[2 * c], s[2 * c + 1]), scale2, base2), e0, e1);
+            const float p0 = ex2(e0), p1 = ex2(e1);
+            sum[c & 1] = add2(sum[c & 1], pack2(p0, p1));
+            p[c] = TT::from_f32(p0, p1);
           }
+          tmem_st_x32(t_buf, p);
           float s0, s1;
           unpack2(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;
           tmem_wait_st();
-        } else if (lane == 0) {
-          mbar_arrive(&B.p_full[grp][0]);
         }
-        ++n_pv;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B.p_full[grp][1]);
+        if (lane == 0) mbar_arrive(&B.p_full[grp][n_tile & 1]);
       }
       if (l != l) m = l;  // a score that is not a number must show in every join
       // ---- the block's end
-      const bool had = first < nt;  // this group had tiles
+      const bool had = first < count;  // this group had tiles
       if (had) {
-        if (!chunk_wait(&B.pv_done[grp], (n_pv - 1) & 1, abort_flag)) goto softmax_out;
+        if (!chunk_wait(&B.o_done[grp], n_out & 1, abort_flag)) goto softmax_out;
+        ++n_out;
         tc_fence_after();
       }
       const bool merge = !pair && nt > 1;
       if (grp == 1 && !pair) {
-        if (had) {
-          // (O goes where Q was: this group's last P V was issued after the block's last Q K^T)
-          if (live) {
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              float o[32];
-              tmem_ld_x32(t_o + c * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int x = 0; x < 32; ++x) sm_o[(c * 32 + x) * 128 + row] = o[x];
-            }
-            sm_ml[row] = m;
-            sm_ml[128 + row] = l;
-          }
+        if (had) {  // the first group reads O itself, out of the same lanes
+          sm_ml[row] = m;
+          sm_ml[128 + row] = l;
           tc_fence_before();
-          fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&B.o_free[1]);
-            mbar_arrive(&B.merge_full);
-          }
+          if (lane == 0) mbar_arrive(&B.merge_full);
         }
         continue;
       }
@@ -616,6 +620,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       if (merge) {
         if (!chunk_wait(&B.merge_full, n_merge & 1, abort_flag)) goto softmax_out;
         ++n_merge;
+        tc_fence_after();
         if (live) {
           const float m1 = sm_ml[row], l1 = sm_ml[128 + row], top = fmaxf(m, m1);
           has1 = m1 != -INFINITY;
@@ -635,33 +640,53 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       float bad = 0.0f;
       if (live) {
         const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
-        T* out = static_cast<T*>(a.out) + static_cast<size_t>(out_row) * a.out_ld + qhead * CHUNK_DIM;
+        const float g0 = f0 * inv, g1 = f1 * inv;
+        uint8_t* stage = sm_out + (warp - 4) * CHUNK_OUT_BYTES;
+        const unsigned rows_valid = __ballot_sync(0xffffffffu, valid);
+        const bool any1 = __any_sync(0xffffffffu, has1);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          float o[32];
+          float o[32], o1[32];
           tmem_ld_x32(t_o + c * 32, o);
+          if (any1) tmem_ld_x32(t_o + 128 + c * 32, o1);
           tmem_wait_ld();
 #pragma unroll
           for (int x = 0; x < 32; ++x) {
-            float v = has0 ? o[x] * f0 : 0.0f;
-            if (has1) v += sm_o[(c * 32 + x) * 128 + row] * f1;
-            v = seen ? v * inv : 0.0f;
+            float v = has0 ? o[x] * g0 : 0.0f;
+            if (has1) v = fmaf(o1[x], g1, v);
+            v = seen ? v : 0.0f;
             bad = fmaf(v, 0.0f, bad);  // NaN once a value is not finite
             o[x] = v;
           }
-          if (valid && whole) {
+          if (!whole) {
+            if (valid)
 #pragma unroll
-            for (int x = 0; x < 32; x += 8) {
-              uint4 v;
-              v.x = TT::from_f32(o[x], o[x + 1]);
-              v.y = TT::from_f32(o[x + 2], o[x + 3]);
-              v.z = TT::from_f32(o[x + 4], o[x + 5]);
-              v.w = TT::from_f32(o[x + 6], o[x + 7]);
-              *reinterpret_cast<uint4*>(out + c * 32 + x) = v;
+              for (int x = 0; x < 32; ++x) part[(c * 32 + x) * CHUNK_PART_ROWS + prow] = o[x];
+            continue;
+          }
+          // through shared memory, so that a store covers whole lines: 64 dims of 4 rows
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint4 v;
+            v.x = TT::from_f32(o[8 * x], o[8 * x + 1]);
+            v.y = TT::from_f32(o[8 * x + 2], o[8 * x + 3]);
+            v.z = TT::from_f32(o[8 * x + 4], o[8 * x + 5]);
+            v.w = TT::from_f32(o[8 * x + 6], o[8 * x + 7]);
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c & 1) * 4 + x) ^ (lane & 7)) * 16)) = v;
+          }
+          if (c & 1) {
+            __syncwarp();
+            for (int y = 0; y < 8; ++y) {
+              const int r = y * 4 + (lane >> 3);
+              if (!(rows_valid >> (y * 4) & 15)) continue;
+              const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
+              if (rows_valid >> r & 1) {
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) * 16));
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
+                                          (c >> 1) * 64 + (lane & 7) * 8) = v;
+              }
             }
-          } else if (valid) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) part[(c * 32 + x) * CHUNK_PART_ROWS + prow] = o[x];
+            __syncwarp();
           }
         }
         if (valid && !whole) {
@@ -670,11 +695,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
       }
       tc_fence_before();
-      if (merge) fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&B.o_free[grp]);
-        if (!pair) mbar_arrive(&B.q_free);
+        if (had) mbar_arrive(&B.o_free[grp]);
+        if (merge) mbar_arrive(&B.o_free[1]);
       }
       // rows that came out not finite, one after the other
       for (unsigned again = __ballot_sync(0xffffffffu, valid && !(bad == 0.0f)); again; again &= again - 1) {
@@ -702,7 +726,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
         }
       }
-      if (!whole && d.t0 == 0 && tid == 0) {
+      if (!whole && d.t0 == 0 && grp == 0 && row == 0) {
         meta->row0 = d.row0;
         meta->ntok = d.ntok;
         meta->head = d.head;
@@ -714,182 +738,170 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       }
     }
   softmax_out:;
-  } else if (warp == 8) {
+  } else if (warp == 0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    // ================================================================ MMA issue
-    constexpr uint32_t id_qk = chunk_idesc<BF16>(false), id_pv = chunk_idesc<BF16>(true);
-    uint32_t n_tile[2] = {0, 0}, n_out[2] = {0, 0}, ring = 0;
-    // S of group g = Q K^T with the key tile at ring position `it`
-    auto scores = [&](int g, uint32_t it, bool pair) {
-      if (elect_one()) {
-        const uint64_t dq = smem_desc_sw128(smem_u32(sm_q) + (pair ? g * CHUNK_STAGE_BYTES : 0));
-        const uint64_t dk = smem_desc_sw128(smem_u32(sm_kv + (it % CHUNK_STAGES) * CHUNK_STAGE_BYTES));
+    // ================================================================ S = Q K^T
+    if (elect_one()) {
+      constexpr uint32_t idesc = chunk_idesc<BF16>(CHUNK_KT, false);
+      uint32_t n_s[2] = {0, 0}, n_q[2] = {0, 0}, st = 0, parity = 0;
+      const uint64_t desc_q = smem_desc_sw128(smem_u32(sm_q)), desc_k = smem_desc_sw128(smem_u32(sm_kv));
+      for (uint32_t n = 0; take_one(n) == 1; ++n) {
+        const ChunkBlock& d = B.block[n % CHUNK_BLOCKS];
+        const int nt = d.nt, nt0 = d.nt0;
+        const bool pair = d.ntok > T_tok;
+        mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
+        const int place = pair ? 0 : n & 1;  // of Q; a pair takes both
+        bool ok = true;
+        for (int x = place; x < (pair ? 2 : place + 1); ++x) ok = ok && wait_one(&B.q_full[x], n_q[x]++ & 1);
+        for (int j = 0; ok && j < nt; ++j) {
+          if (!(ok = wait_one(&B.kv_full[0][st], parity))) break;
+          const uint64_t dk = desc_k + st * (CHUNK_STAGE_BYTES >> 4);
+          // a pair's groups share the key tiles; those of a one-tile block take them in turn
+          for (int g = pair ? static_cast<int>(j >= nt0) : j & 1; g < (pair ? 2 : (j & 1) + 1); ++g) {
+            const uint32_t c = n_s[g]++, buf = c & 1;
+            // the buffer's last P has been read
+            if (c >= 2 && !(ok = wait_one(&B.pv_done[g][buf], ((c >> 1) - 1) & 1))) break;
+            tc_fence_after();
+            const uint64_t dq = desc_q + (pair ? g : place) * (CHUNK_Q_TILE >> 4);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const uint32_t off = ((x >> 2) * CHUNK_HALF_BYTES + (x & 3) * 32) >> 4;
-          umma_f16_ss(tmem + g * 128, dq + off, dk + off, id_qk, x > 0 ? 1u : 0u);
-        }
-        umma_commit(&B.s_full[g]);
-      }
-      __syncwarp();
-    };
-    // O of group g += P V, P by halves as the softmax group hands them over
-    auto values = [&](int g, uint32_t it, bool first) {
-      if (first) {  // the block before has been read out
-        if (n_out[g] && !chunk_wait(&B.o_free[g], (n_out[g] - 1) & 1, abort_flag)) return false;
-        ++n_out[g];
-      }
-      const uint64_t dv = smem_desc_v(smem_u32(sm_kv + (it % CHUNK_STAGES) * CHUNK_STAGE_BYTES));
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (!chunk_wait(&B.p_full[g][h], n_tile[g] & 1, abort_flag)) return false;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int x = h * 4; x < h * 4 + 4; ++x)
-            umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + x * 8, dv + x * (2048 >> 4), id_pv, (!first || x > 0) ? 1u : 0u);
-          if (h == 1) umma_commit(&B.pv_done[g]);
-        }
-        __syncwarp();
-      }
-      ++n_tile[g];
-      return true;
-    };
-    auto release = [&](uint32_t it) {
-      if (elect_one()) umma_commit(&B.kv_free[it % CHUNK_STAGES]);
-      __syncwarp();
-    };
-    auto landed = [&](uint32_t it) {
-      return chunk_wait(&B.kv_full[it % CHUNK_STAGES], (it / CHUNK_STAGES) & 1, abort_flag);
-    };
-    for (uint32_t n_unit = 0; take(n_unit) == 1; ++n_unit) {
-      const ChunkBlock& d = B.block[n_unit % CHUNK_BLOCKS];
-      const int nt = d.nt, t0 = d.t0;
-      const bool pair = d.ntok > T_tok;
-      const int end = d.pos0 + d.ntok;  // positions the block sees
-      give_back(n_unit);
-      if (!chunk_wait(&B.q_full, n_unit & 1, abort_flag)) goto mma_out;
-      // a pair's groups share the key tiles; those of a one-tile block take them in turn
-      if (!landed(ring)) goto mma_out;
-      scores(0, ring, pair);
-      if (pair) {
-        scores(1, ring, pair);
-        release(ring);
-      } else {
-        release(ring);
-        if (nt > 1) {
-          if (!landed(ring + 1)) goto mma_out;
-          scores(1, ring + 1, pair);
-          release(ring + 1);
-        }
-      }
-      if (nt <= (pair ? 1 : 2) && elect_one()) umma_commit(&B.q_free);
-      for (int j = 0; j < nt; ++j) {
-        // ring order: K0 K1 V0 K2 V1 K3 ...
-        const int jn = j + (pair ? 1 : 2);
-        const uint32_t iv = ring + chunk_v_at(j, nt), ik = ring + chunk_k_at(jn);
-        if (pair && jn < nt && !landed(ik)) goto mma_out;
-        if (!landed(iv)) goto mma_out;
-        const int held = end - (t0 + j) * CHUNK_KT;  // positions of this tile that the block sees
-        if (held < CHUNK_KT) {
-          uint8_t* v = sm_kv + (iv % CHUNK_STAGES) * CHUNK_STAGE_BYTES;
-          for (int x = max(held, 0) * 8 + lane; x < CHUNK_KT * 8; x += 32) {
-            reinterpret_cast<uint4*>(v)[x] = make_uint4(0, 0, 0, 0);
-            reinterpret_cast<uint4*>(v + CHUNK_HALF_BYTES)[x] = make_uint4(0, 0, 0, 0);
+            for (int x = 0; x < 8; ++x)
+              umma_f16_ss(tmem + g * 128 + buf * CHUNK_KT, dq + (((x >> 2) * CHUNK_Q_HALF + (x & 3) * 32) >> 4),
+                          dk + (((x >> 2) * CHUNK_HALF_BYTES + (x & 3) * 32) >> 4), idesc, x > 0 ? 1u : 0u);
+            umma_commit(&B.s_full[g][buf]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
+          umma_commit(&B.kv_free[0][st]);
+          if (++st == CHUNK_STAGES) {
+            st = 0;
+            parity ^= 1;
+          }
         }
-        const int g = pair ? 0 : j & 1;
-        if (!values(g, iv, j < (pair ? 1 : 2))) goto mma_out;
-        if (!pair) {
-          release(iv);
-          if (jn < nt && !landed(ik)) goto mma_out;
-        }
-        if (jn < nt) scores(g, ik, pair);
-        if (pair) {
-          if (!values(1, iv, j == 0)) goto mma_out;
-          release(iv);
-          if (jn < nt) scores(1, ik, pair);
-        }
-        if (jn < nt) {
-          release(ik);
-          if (jn == nt - 1 && elect_one()) umma_commit(&B.q_free);
-        }
+        if (!ok) break;
+        for (int x = place; x < (pair ? 2 : place + 1); ++x) umma_commit(&B.q_free[x]);
       }
-      ring += 2 * nt;
     }
-  mma_out:;
-  } else if (warp == 9) {
+    __syncwarp();
+  } else if (warp == 1) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ================================================================ O += P V
+    if (elect_one()) {
+      constexpr uint32_t idesc = chunk_idesc<BF16>(CHUNK_DIM, true);
+      uint32_t n_p[2] = {0, 0}, n_out[2] = {0, 0}, n_clear = 0, st = 0, parity = 0;
+      uint8_t* sm_v = sm_kv + CHUNK_STAGES * CHUNK_STAGE_BYTES;
+      const uint64_t desc_v = smem_desc_v(smem_u32(sm_v));
+      for (uint32_t n = 0; take_one(n) == 1; ++n) {
+        const ChunkBlock& d = B.block[n % CHUNK_BLOCKS];
+        const int nt = d.nt, nt0 = d.nt0, held = d.pos0 + d.ntok - (d.t0 + nt - 1) * CHUNK_KT;  // positions of the last tile
+        const bool pair = d.ntok > T_tok;
+        mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
+        bool ok = true;
+        for (int j = 0; ok && j < nt; ++j) {
+          if (!(ok = wait_one(&B.kv_full[1][st], parity))) break;
+          if (j == nt - 1 && held < CHUNK_KT) {  // behind the block's last position: rows that P's zeros must not meet
+            B.clear_at = sm_v + st * CHUNK_STAGE_BYTES;
+            B.clear_from = max(held, 0);
+            mbar_arrive(&B.clear_ask);
+            if (!(ok = wait_one(&B.clear_done, n_clear++ & 1))) break;
+          }
+          const uint64_t dv = desc_v + st * (CHUNK_STAGE_BYTES >> 4);
+          for (int g = pair ? static_cast<int>(j >= nt0) : j & 1; g < (pair ? 2 : (j & 1) + 1); ++g) {
+            const bool first = pair ? j == 0 : j < 2, last = pair ? j == (g ? nt : nt0) - 1 : j + 2 >= nt;
+            // the block before has been read out
+            if (first && n_out[g]++ && !(ok = wait_one(&B.o_free[g], n_out[g] & 1))) break;
+            const uint32_t c = n_p[g]++, buf = c & 1;
+            if (!(ok = wait_one(&B.p_full[g][buf], (c >> 1) & 1))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + buf * CHUNK_KT + x * 8, dv + x * (2048 >> 4), idesc,
+                          (!first || x > 0) ? 1u : 0u);
+            umma_commit(&B.pv_done[g][buf]);
+            if (last) umma_commit(&B.o_done[g]);
+          }
+          umma_commit(&B.kv_free[1][st]);
+          if (++st == CHUNK_STAGES) {
+            st = 0;
+            parity ^= 1;
+          }
+        }
+        if (!ok) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ================================================================ copies
-    uint32_t ring = 0;
-    for (uint32_t n_unit = 0; take(n_unit) == 1; ++n_unit) {
-      const ChunkBlock& d = B.block[n_unit % CHUNK_BLOCKS];
-      const int ntok = d.ntok, nt = d.nt, t0 = d.t0, row0 = d.row0, head = d.head, slot = d.slot;
-      const bool pair = ntok > T_tok;
-      const int end = d.pos0 + ntok;
-      give_back(n_unit);
-      if (n_unit && !chunk_wait(&B.q_free, (n_unit - 1) & 1, abort_flag)) goto copy_out;
-      if (lane == 0) {
-        const bool small = ntok <= 8;
-        const int tiles = pair ? 2 : 1;
-        mbar_arrive_expect_tx(&B.q_full, tiles * 2 * (small ? 8 : T_tok) * group * 128);
-        for (int x = 0; x < tiles; ++x)
-          for (int h = 0; h < 2; ++h)
-            tma_load_4d(sm_q + x * CHUNK_STAGE_BYTES + h * CHUNK_HALF_BYTES, small ? &q_small : &q_big, &B.q_full, 0,
-                        head * group, row0 + x * T_tok, h);
-      }
-      __syncwarp();
-      const int pages = min((max(end, 0) + CHUNK_PAGE - 1) / CHUNK_PAGE, 2 * (t0 + nt));  // of the range, from page 0 on
-      int page_of = 0, from = -1;
-      for (int x = 0; x < 2 * nt; ++x) {
-        // ring order: K0 K1 V0 K2 V1 ...
-        const bool is_v = nt == 1 ? x == 1 : x == 2 * nt - 1 || (x > 1 && (x & 1) == 0);
-        const int j = x == 2 * nt - 1 ? nt - 1 : is_v ? (x - 2) / 2 : (x + 1) / 2;
-        const int p0 = 2 * (t0 + j), have = min(2, pages - p0);
-        if (from < 0 || p0 < from || p0 + 2 > from + 32) {  // page ids, 32 at a time
-          from = is_v ? p0 : max(p0 - 4, 0);
-          page_of = from + lane < pages ? a.page_table[static_cast<size_t>(slot) * a.max_pages + from + lane] : -1;
-        }
-        const uint32_t it = ring + x, st = it % CHUNK_STAGES;
-        if (it >= CHUNK_STAGES && !chunk_wait(&B.kv_free[st], (it / CHUNK_STAGES - 1) & 1, abort_flag)) goto copy_out;
-        const int pg0 = __shfl_sync(0xffffffffu, page_of, (p0 - from) & 31), pg1 = __shfl_sync(0xffffffffu, page_of, (p0 + 1 - from) & 31);
-        if (lane == 0) {
-          uint8_t* dst = sm_kv + st * CHUNK_STAGE_BYTES;
-          if (have > 0) mbar_arrive_expect_tx(&B.kv_full[st], have * CHUNK_PAGE * CHUNK_DIM * 2);
-          else mbar_arrive(&B.kv_full[st]);
-          for (int y = 0; y < have; ++y) {
-            const int page = y ? pg1 : pg0;
-            // a page outside the pool reads as zeros: rows behind the map's last
-            const int r = page < 0 || page >= a.pool_pages
-                              ? a.pool_pages * a.layers * 2 * a.nkv * CHUNK_PAGE
-                              : (((page * a.layers + a.layer) * 2 + (is_v ? 1 : 0)) * a.nkv + head) * CHUNK_PAGE;
+    if (elect_one()) {
+      uint32_t n_q[2] = {0, 0}, st[2] = {0, 0}, lap[2] = {0, 0};  // of K and V
+      const int no_row = a.pool_pages * a.layers * 2 * a.nkv * CHUNK_PAGE;  // behind the map's last row: reads as zeros
+      const int page_rows = a.layers * 2 * a.nkv * CHUNK_PAGE;
+      bool ok = true;
+      for (uint32_t n = 0; ok && take_one(n) == 1; ++n) {
+        const ChunkBlock& d = B.block[n % CHUNK_BLOCKS];
+        const int ntok = d.ntok, nt = d.nt, t0 = d.t0, row0 = d.row0, head = d.head;
+        const bool pair = ntok > T_tok, small = ntok <= 8;
+        // pages that hold anything the block sees
+        const int have = min((max(d.pos0 + ntok, 0) + CHUNK_PAGE - 1) / CHUNK_PAGE - t0, nt);
+        const int* table = a.page_table + static_cast<size_t>(max(d.slot, 0)) * a.max_pages + t0;
+        const int row_k = (a.layer * 2 * a.nkv + head) * CHUNK_PAGE, row_v = row_k + a.nkv * CHUNK_PAGE;
+        auto load_q = [&] {
+          for (int x = pair ? 0 : n & 1; x < (pair ? 2 : static_cast<int>(n & 1) + 1); ++x) {
+            if (n_q[x]++ && !wait_one(&B.q_free[x], n_q[x] & 1)) return false;
+            mbar_arrive_expect_tx(&B.q_full[x], 2 * (small ? 8 : T_tok) * group * 128);
             for (int h = 0; h < 2; ++h)
-              tma_load_3d(dst + h * CHUNK_HALF_BYTES + y * (CHUNK_PAGE * 128), &kv_map, &B.kv_full[st], 0, r, h);
+              tma_load_4d(sm_q + x * CHUNK_Q_TILE + h * CHUNK_Q_HALF, small ? &q_small : &q_big, &B.q_full[x], 0, head * group,
+                          row0 + (pair ? x * T_tok : 0), h);
           }
+          return true;
+        };
+        auto load_page = [&](int v, int page, bool there) {
+          if (lap[v] && !wait_one(&B.kv_free[v][st[v]], (lap[v] - 1) & 1)) return false;
+          uint64_t* bar = &B.kv_full[v][st[v]];
+          if (there) {
+            const int r = page < 0 || page >= a.pool_pages ? no_row : page * page_rows + (v ? row_v : row_k);
+            mbar_arrive_expect_tx(bar, CHUNK_STAGE_BYTES);
+            tma_load_3d(sm_kv + (v * CHUNK_STAGES + st[v]) * CHUNK_STAGE_BYTES, &kv_map, bar, 0, r, 0);
+          } else {
+            mbar_arrive(bar);
+          }
+          if (++st[v] == CHUNK_STAGES) {
+            st[v] = 0;
+            ++lap[v];
+          }
+          return true;
+        };
+        // K runs two tiles ahead of V: K0 K1 K2 V0 K3 V1 ...  Q goes first where its place is free (one row tile: the
+        // places alternate), else behind the first K, whose stages free up with the block before.
+        if (!pair) ok = load_q();
+        int id0 = -1, id1 = -1, id2 = -1, next = have > 0 ? d.pages[0] : -1;
+        for (int j = 0; ok && j < nt + 2; ++j) {
+          id0 = id1;
+          id1 = id2;
+          id2 = next;
+          if (j < nt) {
+            if (j + 1 < have) next = j + 1 < 16 ? d.pages[j + 1] : __ldg(table + j + 1);
+            ok = load_page(0, id2, j < have);
+            if (ok && pair && j == 0) ok = load_q();
+          }
+          if (ok && j >= 2) ok = load_page(1, id0, j - 2 < have);
         }
-        __syncwarp();
+        mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
       }
-      ring += 2 * nt;
-    }
-  copy_out:
-    if (*abort_flag && lane == 0) {
-      // copies still in flight land before the shared memory is given back: the newest of each stage, bounded
-      const uint64_t t0 = globaltimer();
-      for (int st = 0; st < CHUNK_STAGES; ++st)
-        for (uint32_t x = 0; x < 2; ++x)
-          while (!mbar_try_wait(&B.kv_full[st], x) && globaltimer() - t0 < 20000000ull) {
+      if (*abort_flag) {
+        // copies still in flight land before the shared memory is given back: the newest of each stage, bounded
+        const uint64_t t0 = globaltimer();
+        for (int x = 0; x < 2 * CHUNK_STAGES; ++x)
+          for (uint32_t y = 0; y < 2; ++y)
+            while (!mbar_try_wait(&B.kv_full[0][0] + x, y) && globaltimer() - t0 < 20000000ull) {
+            }
+        for (uint32_t x = 0; x < 4; ++x)
+          while (!mbar_try_wait(&B.q_full[x >> 1], x & 1) && globaltimer() - t0 < 40000000ull) {
           }
-      for (uint32_t x = 0; x < 2; ++x)
-        while (!mbar_try_wait(&B.q_full, x) && globaltimer() - t0 < 40000000ull) {
-        }
+      }
     }
-  } else if (warp == 11) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    __syncwarp();
   } else {
-    // ================================================================ the walk
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ================================================================ the walk
     ChunkWalk w;
     bool more = B.any != 0;
     if (more) {
@@ -903,27 +915,50 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       w.nb = (w.s.n + bt - 1) / bt;
       more = chunk_fit(a, w, bt);
     }
+    // Block n is handed on while block n - 1 is worked at; then comes the clearing for block n - 1, so nothing that a
+    // block waits for ever stands behind a wait for that block.
+    uint32_t n_clear = 0;
+    bool clear = false, clear_before = false;  // block n, n - 1 wants V rows cleared
     for (uint32_t n = 0;; ++n) {
       if (n >= CHUNK_BLOCKS && !chunk_wait(&B.block_free[n % CHUNK_BLOCKS], (n / CHUNK_BLOCKS - 1) & 1, abort_flag)) break;
-      if (lane == 0) {
-        ChunkBlock& d = B.block[n % CHUNK_BLOCKS];
-        d.more = more;
-        if (more) {
-          const int tok0 = w.k * bt;
+      ChunkBlock& d = B.block[n % CHUNK_BLOCKS];
+      if (more) {
+        const int tok0 = w.k * bt, pos0 = w.s.len - w.s.n + tok0, ntok = min(w.s.n - tok0, bt), end = pos0 + ntok;
+        const int have = min((max(end, 0) + CHUNK_PAGE - 1) / CHUNK_PAGE, w.t1);
+        if (lane < 16)
+          d.pages[lane] = w.t0 + lane < have ? a.page_table[static_cast<size_t>(w.s.slot) * a.max_pages + w.t0 + lane] : -1;
+        clear = end - (w.t1 - 1) * CHUNK_KT < CHUNK_KT;
+        if (lane == 0) {
           d.row0 = w.s.row0 + tok0;
-          d.ntok = min(w.s.n - tok0, bt);
-          d.pos0 = w.s.len - w.s.n + tok0;
+          d.ntok = ntok;
+          d.pos0 = pos0;
           d.head = w.g;
           d.slot = w.s.slot;
           d.t0 = w.t0;
           d.nt = w.t1 - w.t0;
           d.tiles = w.nt;
+          d.nt0 = min(max((pos0 + T_tok + CHUNK_KT - 1) / CHUNK_KT - w.t0, 0), d.nt);  // (0 where nothing is seen)
           d.base = w.base;
         }
-        mbar_arrive(&B.block_full[n % CHUNK_BLOCKS]);
       }
       __syncwarp();
+      if (lane == 0) {
+        d.more = more;
+        mbar_arrive(&B.block_full[n % CHUNK_BLOCKS]);
+      }
+      if (clear_before) {
+        if (!chunk_wait(&B.clear_ask, n_clear++ & 1, abort_flag)) break;
+        uint8_t* v = B.clear_at;
+        for (int x = B.clear_from * 8 + lane; x < CHUNK_KT * 8; x += 32) {
+          reinterpret_cast<uint4*>(v)[x] = make_uint4(0, 0, 0, 0);
+          reinterpret_cast<uint4*>(v + CHUNK_HALF_BYTES)[x] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.clear_done);
+      }
       if (!more) break;
+      clear_before = clear;
       more = chunk_next(a, w, bt);
     }
   }
@@ -931,7 +966,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   if (tid == 0 && B.abort_flag) meta->state = 2;
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
 // Joins the partials of the block that CTA blockIdx.x began and others went on with; blockIdx.y takes

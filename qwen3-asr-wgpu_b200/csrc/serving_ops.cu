@@ -264,14 +264,14 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
   const uint64_t kv_rows = static_cast<uint64_t>(pool_pages) * layers * 2 * nkv * CHUNK_PAGE;
   // Q as {64 dims, heads, rows, 2 halves}: a box is one half of a group's heads of some rows, in the order in which
   // a row tile packs them, under the tensor core's 128-byte swizzle.  The cache as {64 dims, rows, 2
-  // halves}: a box is one half of a page, copied as it is (its rows are swizzled already).
+  // halves}: a box is a page, half after half, copied as it is (its rows are swizzled already).
   CUtensorMap q_big, q_small, kv_map;
   const cuuint64_t q_dims[4] = {64, static_cast<cuuint64_t>(nq), static_cast<cuuint64_t>(rows), 2};
   const cuuint64_t q_strides[3] = {CHUNK_DIM * 2, static_cast<cuuint64_t>(q_ld) * 2, 128};
   const cuuint32_t big[4] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(chunk_tile_tokens(group)), 1};
   const cuuint32_t small[4] = {64, static_cast<cuuint32_t>(group), 8, 1};
   const cuuint64_t kv_dims[3] = {64, kv_rows, 2}, kv_strides[2] = {CHUNK_DIM * 2, 128};
-  const cuuint32_t kv_box[3] = {64, CHUNK_PAGE, 1};
+  const cuuint32_t kv_box[3] = {64, CHUNK_PAGE, 2};
   if (!encode_map(&q_big, q, 4, q_dims, q_strides, big, true) || !encode_map(&q_small, q, 4, q_dims, q_strides, small, true) ||
       !encode_map(&kv_map, kv_pool, 3, kv_dims, kv_strides, kv_box, false))
     return op_err(err, errlen, QASR_ERR_DEVICE, "chunk attention tensor maps");
