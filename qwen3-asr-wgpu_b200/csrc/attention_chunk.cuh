@@ -57,6 +57,7 @@ struct ChunkArgs {
   int pool_pages;
   const int* page_table;
   int max_slots, max_pages, layers, nq, nkv, layer;
+  int group, tile_tokens;  // nq / nkv; tokens of a row tile (chunk_tile_tokens)
   const int* seq_slot;
   const int* cu_rows;
   const int* kv_len;
@@ -68,13 +69,13 @@ struct ChunkArgs {
 
 constexpr int CHUNK_THREADS = 384;
 constexpr int CHUNK_KT = CHUNK_PAGE;              // keys per tile
-constexpr int CHUNK_STAGES = 4;                   // of K and of V each
+constexpr int CHUNK_K_STAGES = 4, CHUNK_V_STAGES = 5;  // V is held until its P is there
 constexpr int CHUNK_STAGE_BYTES = CHUNK_KT * CHUNK_DIM * 2;
 constexpr int CHUNK_HALF_BYTES = CHUNK_KT * 128;  // the rows' first or second 64 dims
 constexpr int CHUNK_Q_TILE = 128 * CHUNK_DIM * 2, CHUNK_Q_HALF = CHUNK_Q_TILE / 2;
 constexpr int CHUNK_Q_BYTES = 2 * CHUNK_Q_TILE;
-constexpr int CHUNK_OUT_BYTES = 32 * 128;          // per softmax warp: half of its rows' output
-constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + 2 * CHUNK_STAGES * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 2048;
+constexpr int CHUNK_OUT_BYTES = 32 * 64;           // per softmax warp: a quarter of its rows' output
+constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 2048;
 constexpr int CHUNK_BLOCK_COST = 2;               // a block's Q copy, first and last steps, in key tiles
 constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
@@ -142,17 +143,22 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkArgs& a, int i) {
 }
 // key tiles of block k (rows [k * bt, min(n, (k + 1) * bt)) of the request): at least one, so that a
 // block which sees nothing is visited and written
+__device__ __forceinline__ int chunk_blocks(int n, int bt) { return n <= bt ? (n > 0) : (n + bt - 1) / bt; }
 __device__ __forceinline__ int chunk_tiles(const ChunkSeq& s, int k, int bt) {
   const int end = s.len - s.n + min(s.n, (k + 1) * bt);
   return max(1, (end + CHUNK_KT - 1) / CHUNK_KT);
 }
 __device__ __forceinline__ long long chunk_head_cost(const ChunkSeq& s, int bt) {
   long long c = 0;
-  const int nb = (s.n + bt - 1) / bt;
+  const int nb = chunk_blocks(s.n, bt);
   for (int k = 0; k < nb; ++k) c += chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST;
   return c;
 }
-__device__ __forceinline__ long long chunk_bound(long long total, int c, int grid) { return total * c / grid; }
+__device__ __forceinline__ long long chunk_bound(long long total, int c, int grid) {
+  if (total < (1 << 22))  // (grid <= 512) a 64-bit division is a slow routine
+    return static_cast<uint32_t>(total) * static_cast<uint32_t>(c) / static_cast<uint32_t>(grid);
+  return total * c / grid;
+}
 // The first key tile behind cut x of a block that starts at `base`.
 __device__ __forceinline__ int chunk_cut(long long x, long long base, int nt) {
   const long long t = x - base - CHUNK_BLOCK_COST;
@@ -182,7 +188,7 @@ __device__ __forceinline__ bool chunk_fit(const ChunkArgs& a, ChunkWalk& w, int 
           if (++w.i >= a.n_seqs) return false;
           w.s = chunk_seq(a, w.i);
         } while (w.s.n == 0);
-        w.nb = (w.s.n + bt - 1) / bt;
+        w.nb = chunk_blocks(w.s.n, bt);
       }
     }
   }
@@ -198,7 +204,7 @@ __device__ __forceinline__ bool chunk_next(const ChunkArgs& a, ChunkWalk& w, int
         if (++w.i >= a.n_seqs) return false;
         w.s = chunk_seq(a, w.i);
       } while (w.s.n == 0);
-      w.nb = (w.s.n + bt - 1) / bt;
+      w.nb = chunk_blocks(w.s.n, bt);
     }
   }
   return chunk_fit(a, w, bt);
@@ -316,7 +322,7 @@ __device__ __noinline__ void chunk_row(const ChunkArgs& a, int slot, int row, in
                                        float& m, float& l, float4& o) {
   using TT = ChunkType<BF16>;
   using T = typename TT::T;
-  const int lane = threadIdx.x & 31, head = qhead / (a.nq / a.nkv);
+  const int lane = threadIdx.x & 31, head = qhead / a.group;
   const uint2 qv = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) + static_cast<size_t>(row) * a.q_ld +
                                                    qhead * CHUNK_DIM + lane * 4);
   const float2 q01 = TT::to_f32(qv.x), q23 = TT::to_f32(qv.y);
@@ -365,7 +371,7 @@ constexpr int CHUNK_BLOCKS = 3;
 
 struct ChunkBars {
   uint64_t q_full[2], q_free[2];               // of a row tile's place
-  uint64_t kv_full[2][CHUNK_STAGES], kv_free[2][CHUNK_STAGES];  // K, V
+  uint64_t kv_full[CHUNK_K_STAGES + CHUNK_V_STAGES], kv_free[CHUNK_K_STAGES + CHUNK_V_STAGES];  // of K, then of V
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_done[2], o_free[2], merge_full;
   uint64_t clear_ask, clear_done;              // rows of a V stage to be zeroed
   uint8_t* clear_at;
@@ -376,7 +382,8 @@ struct ChunkBars {
   int abort_flag;
   // the range's first block
   int i, g, k, any;
-  long long base, total;
+  ChunkSeq seq;
+  long long base;
   long long scan[CHUNK_THREADS / 32];
 };
 static_assert(sizeof(ChunkBars) <= 1024, "ChunkBars sits in the last KB of the shared memory");
@@ -391,22 +398,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(chunk_dsmem) + 1023) & ~uintptr_t(1023));
   uint8_t* sm_q = smem;                                    // two row tiles, each [2 halves][128 rows][128 B]
   uint8_t* sm_kv = smem + CHUNK_Q_BYTES;                   // stages of K, then of V: [2 halves][64 positions][128 B]
-  uint8_t* sm_out = sm_kv + 2 * CHUNK_STAGES * CHUNK_STAGE_BYTES;  // per softmax warp [32 rows][128 B], chunks of 16 B swizzled
+  uint8_t* sm_out = sm_kv + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES;  // per softmax warp [32 rows][64 B], chunks swizzled
   float* sm_ml = reinterpret_cast<float*>(sm_out + 8 * CHUNK_OUT_BYTES);  // [2][128]: group 1's m and l
   ChunkBars& B = *reinterpret_cast<ChunkBars*>(reinterpret_cast<uint8_t*>(sm_ml) + 1024);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grid = gridDim.x, cta = blockIdx.x;
-  const int group = a.nq / a.nkv, T_tok = chunk_tile_tokens(group), bt = 2 * T_tok;
+  const int group = a.group, T_tok = a.tile_tokens, bt = 2 * T_tok;
 
   if (tid == 0) {
     mbar_init(&B.clear_ask, 1);
     mbar_init(&B.clear_done, 1);
-    for (int i = 0; i < CHUNK_STAGES; ++i) {
-      for (int x = 0; x < 2; ++x) {
-        mbar_init(&B.kv_full[x][i], 1);
-        mbar_init(&B.kv_free[x][i], 1);
-      }
+    for (int i = 0; i < CHUNK_K_STAGES + CHUNK_V_STAGES; ++i) {
+      mbar_init(&B.kv_full[i], 1);
+      mbar_init(&B.kv_free[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B.s_full[i][0], 1);
@@ -445,7 +450,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   const int per = (a.n_seqs + CHUNK_THREADS - 1) / CHUNK_THREADS;
   const int i0 = min(tid * per, a.n_seqs), i1 = min(i0 + per, a.n_seqs);
   long long mine = 0;
-  for (int i = i0; i < i1; ++i) mine += chunk_head_cost(chunk_seq(a, i), bt) * a.nkv;
+  ChunkSeq s{};
+  long long head_cost = 0;  // (of the thread's only request, in most calls)
+  for (int i = i0; i < i1; ++i) {
+    s = chunk_seq(a, i);
+    head_cost = chunk_head_cost(s, bt);
+    mine += head_cost * a.nkv;
+  }
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -465,17 +476,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   if (lo < hi && incl - mine <= lo && lo < incl) {
     long long base = incl - mine;
     int i = i0;
-    ChunkSeq s;
-    long long head_cost;
-    while (true) {
+    while (per > 1) {
       s = chunk_seq(a, i);
       head_cost = chunk_head_cost(s, bt);
       if (lo < base + head_cost * a.nkv) break;
       base += head_cost * a.nkv;
       ++i;
     }
-    const int g = static_cast<int>((lo - base) / head_cost);
-    base += g * head_cost;
+    int g = 0;
+    for (; lo >= base + head_cost; ++g) base += head_cost;
     int k = 0;
     while (lo >= base + chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST) {
       base += chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST;
@@ -485,6 +494,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     B.g = g;
     B.k = k;
     B.base = base;
+    B.seq = s;
     B.any = 1;
   }
   __syncthreads();
@@ -664,7 +674,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               for (int x = 0; x < 32; ++x) part[(c * 32 + x) * CHUNK_PART_ROWS + prow] = o[x];
             continue;
           }
-          // through shared memory, so that a store covers whole lines: 64 dims of 4 rows
+          // through shared memory, so that a store covers whole sectors: 32 dims of 8 rows
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             uint4 v;
@@ -672,22 +682,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             v.y = TT::from_f32(o[8 * x + 2], o[8 * x + 3]);
             v.z = TT::from_f32(o[8 * x + 4], o[8 * x + 5]);
             v.w = TT::from_f32(o[8 * x + 6], o[8 * x + 7]);
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c & 1) * 4 + x) ^ (lane & 7)) * 16)) = v;
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((x ^ (lane >> 1 & 3)) * 16)) = v;
           }
-          if (c & 1) {
-            __syncwarp();
-            for (int y = 0; y < 8; ++y) {
-              const int r = y * 4 + (lane >> 3);
-              if (!(rows_valid >> (y * 4) & 15)) continue;
-              const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
-              if (rows_valid >> r & 1) {
-                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) * 16));
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
-                                          (c >> 1) * 64 + (lane & 7) * 8) = v;
-              }
+          __syncwarp();
+          for (int y = 0; y < 4; ++y) {
+            const int r = y * 8 + (lane >> 2);
+            if (!(rows_valid >> (y * 8) & 255)) continue;
+            const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
+            if (rows_valid >> r & 1) {
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) * 16));
+              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
+                                        c * 32 + (lane & 3) * 8) = v;
             }
-            __syncwarp();
           }
+          __syncwarp();
         }
         if (valid && !whole) {
           part[CHUNK_DIM * CHUNK_PART_ROWS + prow] = m;
@@ -754,7 +762,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         bool ok = true;
         for (int x = place; x < (pair ? 2 : place + 1); ++x) ok = ok && wait_one(&B.q_full[x], n_q[x]++ & 1);
         for (int j = 0; ok && j < nt; ++j) {
-          if (!(ok = wait_one(&B.kv_full[0][st], parity))) break;
+          if (!(ok = wait_one(&B.kv_full[st], parity))) break;
           const uint64_t dk = desc_k + st * (CHUNK_STAGE_BYTES >> 4);
           // a pair's groups share the key tiles; those of a one-tile block take them in turn
           for (int g = pair ? static_cast<int>(j >= nt0) : j & 1; g < (pair ? 2 : (j & 1) + 1); ++g) {
@@ -769,8 +777,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                           dk + (((x >> 2) * CHUNK_HALF_BYTES + (x & 3) * 32) >> 4), idesc, x > 0 ? 1u : 0u);
             umma_commit(&B.s_full[g][buf]);
           }
-          umma_commit(&B.kv_free[0][st]);
-          if (++st == CHUNK_STAGES) {
+          umma_commit(&B.kv_free[st]);
+          if (++st == CHUNK_K_STAGES) {
             st = 0;
             parity ^= 1;
           }
@@ -786,7 +794,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     if (elect_one()) {
       constexpr uint32_t idesc = chunk_idesc<BF16>(CHUNK_DIM, true);
       uint32_t n_p[2] = {0, 0}, n_out[2] = {0, 0}, n_clear = 0, st = 0, parity = 0;
-      uint8_t* sm_v = sm_kv + CHUNK_STAGES * CHUNK_STAGE_BYTES;
+      uint8_t* sm_v = sm_kv + CHUNK_K_STAGES * CHUNK_STAGE_BYTES;
       const uint64_t desc_v = smem_desc_v(smem_u32(sm_v));
       for (uint32_t n = 0; take_one(n) == 1; ++n) {
         const ChunkBlock& d = B.block[n % CHUNK_BLOCKS];
@@ -795,7 +803,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
         bool ok = true;
         for (int j = 0; ok && j < nt; ++j) {
-          if (!(ok = wait_one(&B.kv_full[1][st], parity))) break;
+          if (!(ok = wait_one(&B.kv_full[CHUNK_K_STAGES + st], parity))) break;
           if (j == nt - 1 && held < CHUNK_KT) {  // behind the block's last position: rows that P's zeros must not meet
             B.clear_at = sm_v + st * CHUNK_STAGE_BYTES;
             B.clear_from = max(held, 0);
@@ -817,8 +825,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             umma_commit(&B.pv_done[g][buf]);
             if (last) umma_commit(&B.o_done[g]);
           }
-          umma_commit(&B.kv_free[1][st]);
-          if (++st == CHUNK_STAGES) {
+          umma_commit(&B.kv_free[CHUNK_K_STAGES + st]);
+          if (++st == CHUNK_V_STAGES) {
             st = 0;
             parity ^= 1;
           }
@@ -831,7 +839,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ================================================================ copies
     if (elect_one()) {
-      uint32_t n_q[2] = {0, 0}, st[2] = {0, 0}, lap[2] = {0, 0};  // of K and V
+      uint32_t n_q0 = 0, n_q1 = 0, st_k = 0, lap_k = 0, st_v = 0, lap_v = 0;
       const int no_row = a.pool_pages * a.layers * 2 * a.nkv * CHUNK_PAGE;  // behind the map's last row: reads as zeros
       const int page_rows = a.layers * 2 * a.nkv * CHUNK_PAGE;
       bool ok = true;
@@ -843,35 +851,29 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const int have = min((max(d.pos0 + ntok, 0) + CHUNK_PAGE - 1) / CHUNK_PAGE - t0, nt);
         const int* table = a.page_table + static_cast<size_t>(max(d.slot, 0)) * a.max_pages + t0;
         const int row_k = (a.layer * 2 * a.nkv + head) * CHUNK_PAGE, row_v = row_k + a.nkv * CHUNK_PAGE;
-        auto load_q = [&] {
-          for (int x = pair ? 0 : n & 1; x < (pair ? 2 : static_cast<int>(n & 1) + 1); ++x) {
-            if (n_q[x]++ && !wait_one(&B.q_free[x], n_q[x] & 1)) return false;
-            mbar_arrive_expect_tx(&B.q_full[x], 2 * (small ? 8 : T_tok) * group * 128);
-            for (int h = 0; h < 2; ++h)
-              tma_load_4d(sm_q + x * CHUNK_Q_TILE + h * CHUNK_Q_HALF, small ? &q_small : &q_big, &B.q_full[x], 0, head * group,
-                          row0 + (pair ? x * T_tok : 0), h);
-          }
+        auto load_q = [&](int x, uint32_t& used) {
+          if (used && !wait_one(&B.q_free[x], (used - 1) & 1)) return false;
+          ++used;
+          mbar_arrive_expect_tx(&B.q_full[x], 2 * (small ? 8 : T_tok) * group * 128);
+          for (int h = 0; h < 2; ++h)
+            tma_load_4d(sm_q + x * CHUNK_Q_TILE + h * CHUNK_Q_HALF, small ? &q_small : &q_big, &B.q_full[x], 0, head * group,
+                        row0 + (pair ? x * T_tok : 0), h);
           return true;
         };
-        auto load_page = [&](int v, int page, bool there) {
-          if (lap[v] && !wait_one(&B.kv_free[v][st[v]], (lap[v] - 1) & 1)) return false;
-          uint64_t* bar = &B.kv_full[v][st[v]];
+        auto load_page = [&](int at, uint32_t lap, int page, int row_of, bool there) {
+          if (lap && !wait_one(&B.kv_free[at], (lap - 1) & 1)) return false;
           if (there) {
-            const int r = page < 0 || page >= a.pool_pages ? no_row : page * page_rows + (v ? row_v : row_k);
-            mbar_arrive_expect_tx(bar, CHUNK_STAGE_BYTES);
-            tma_load_3d(sm_kv + (v * CHUNK_STAGES + st[v]) * CHUNK_STAGE_BYTES, &kv_map, bar, 0, r, 0);
+            mbar_arrive_expect_tx(&B.kv_full[at], CHUNK_STAGE_BYTES);
+            tma_load_3d(sm_kv + at * CHUNK_STAGE_BYTES, &kv_map, &B.kv_full[at], 0,
+                        page < 0 || page >= a.pool_pages ? no_row : page * page_rows + row_of, 0);
           } else {
-            mbar_arrive(bar);
-          }
-          if (++st[v] == CHUNK_STAGES) {
-            st[v] = 0;
-            ++lap[v];
+            mbar_arrive(&B.kv_full[at]);
           }
           return true;
         };
         // K runs two tiles ahead of V: K0 K1 K2 V0 K3 V1 ...  Q goes first where its place is free (one row tile: the
         // places alternate), else behind the first K, whose stages free up with the block before.
-        if (!pair) ok = load_q();
+        if (!pair) ok = n & 1 ? load_q(1, n_q1) : load_q(0, n_q0);
         int id0 = -1, id1 = -1, id2 = -1, next = have > 0 ? d.pages[0] : -1;
         for (int j = 0; ok && j < nt + 2; ++j) {
           id0 = id1;
@@ -879,19 +881,29 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           id2 = next;
           if (j < nt) {
             if (j + 1 < have) next = j + 1 < 16 ? d.pages[j + 1] : __ldg(table + j + 1);
-            ok = load_page(0, id2, j < have);
-            if (ok && pair && j == 0) ok = load_q();
+            ok = load_page(st_k, lap_k, id2, row_k, j < have);
+            if (++st_k == CHUNK_K_STAGES) {
+              st_k = 0;
+              ++lap_k;
+            }
+            if (ok && pair && j == 0) ok = load_q(0, n_q0) && load_q(1, n_q1);
           }
-          if (ok && j >= 2) ok = load_page(1, id0, j - 2 < have);
+          if (ok && j >= 2) {
+            ok = load_page(CHUNK_K_STAGES + st_v, lap_v, id0, row_v, j - 2 < have);
+            if (++st_v == CHUNK_V_STAGES) {
+              st_v = 0;
+              ++lap_v;
+            }
+          }
         }
         mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
       }
       if (*abort_flag) {
         // copies still in flight land before the shared memory is given back: the newest of each stage, bounded
         const uint64_t t0 = globaltimer();
-        for (int x = 0; x < 2 * CHUNK_STAGES; ++x)
+        for (int x = 0; x < CHUNK_K_STAGES + CHUNK_V_STAGES; ++x)
           for (uint32_t y = 0; y < 2; ++y)
-            while (!mbar_try_wait(&B.kv_full[0][0] + x, y) && globaltimer() - t0 < 20000000ull) {
+            while (!mbar_try_wait(&B.kv_full[x], y) && globaltimer() - t0 < 20000000ull) {
             }
         for (uint32_t x = 0; x < 4; ++x)
           while (!mbar_try_wait(&B.q_full[x >> 1], x & 1) && globaltimer() - t0 < 40000000ull) {
@@ -911,8 +923,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       w.base = B.base;
       w.lo = lo;
       w.hi = hi;
-      w.s = chunk_seq(a, w.i);
-      w.nb = (w.s.n + bt - 1) / bt;
+      w.s = B.seq;
+      w.nb = chunk_blocks(w.s.n, bt);
       more = chunk_fit(a, w, bt);
     }
     // Block n is handed on while block n - 1 is worked at; then comes the clearing for block n - 1, so nothing that a
@@ -979,7 +991,7 @@ __global__ void __launch_bounds__(256) attention_chunk_combine_kernel(const __gr
   griddep_launch_dependents();
   const ChunkMeta* meta = reinterpret_cast<const ChunkMeta*>(a.ws + static_cast<size_t>(blockIdx.x) * 64);
   if (meta->state != 1) return;
-  const int group = a.nq / a.nkv, T_tok = chunk_tile_tokens(group);
+  const int group = a.group, T_tok = a.tile_tokens;
   const int prow = blockIdx.y * 32 + (threadIdx.x & 31), col = (threadIdx.x >> 5) * 16;
   const int tok = (prow >> 7) * T_tok + (prow & 127) / group, head = meta->head * group + (prow & 127) % group;
   if ((prow & 127) >= T_tok * group || tok >= meta->ntok) return;

@@ -255,7 +255,7 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
   DeviceScope dev(device);
   if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
   const int grid = sm_count(device);
-  if (grid <= 0) return op_err(err, errlen, QASR_ERR_DEVICE, "device attributes");
+  if (grid <= 0 || grid > 512) return op_err(err, errlen, QASR_ERR_DEVICE, "device attributes");
   if (ws_bytes < chunk_ws_bytes(grid))
     return op_err(err, errlen, QASR_ERR_CAPACITY, "chunk attention workspace too small");
   cudaError_t e = chunk_attrs(device);
@@ -278,13 +278,14 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
   // a scale of 0 becomes a tiny one: masked scores stay -inf under it, and every other score still counts alike
   const float s2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
   const ChunkArgs a{q, q_ld, out, out_ld, rows, kv_pool, pool_pages, page_table, max_slots, max_pages, layers, nq, nkv,
-                    layer, seq_slot, cu_rows, kv_len, n_seqs, s2, scale < 0.0f, static_cast<uint8_t*>(ws)};
+                    layer, group, chunk_tile_tokens(group), seq_slot, cu_rows, kv_len, n_seqs, s2, scale < 0.0f, static_cast<uint8_t*>(ws)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = type == QASR_TYPE_BF16;
   e = bf ? launch_k(attention_chunk_kernel<true>, dim3(grid), dim3(CHUNK_THREADS), CHUNK_SMEM, st, true, q_big, q_small, kv_map, a)
          : launch_k(attention_chunk_kernel<false>, dim3(grid), dim3(CHUNK_THREADS), CHUNK_SMEM, st, true, q_big, q_small, kv_map, a);
   if (e != cudaSuccess) return op_cuda(err, errlen, e, "chunk attention launch");
-  const dim3 cgrid(grid, CHUNK_PART_ROWS / 32);
+  // 32 of a block's packed rows each; no block has more rows than the call
+  const dim3 cgrid(grid, rows <= chunk_tile_tokens(group) ? (rows * group + 31) / 32 : CHUNK_PART_ROWS / 32);
   e = bf ? launch_k(attention_chunk_combine_kernel<true>, cgrid, dim3(256), 0, st, true, a, grid)
          : launch_k(attention_chunk_combine_kernel<false>, cgrid, dim3(256), 0, st, true, a, grid);
   return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "chunk attention combine launch");
