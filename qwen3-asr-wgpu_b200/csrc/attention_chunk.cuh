@@ -81,12 +81,15 @@ constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block'
 constexpr float CHUNK_RESCALE = 8.0f;
 constexpr uint32_t CHUNK_WAIT_STEPS = (10 * QASR_WAIT_NS) >> 20;  // rows computed again by chunk_row keep the others waiting
 constexpr int CHUNK_PART_ROWS = 256;
-constexpr int CHUNK_PART_FLOATS = (CHUNK_DIM + 2) * CHUNK_PART_ROWS;  // [o 0..127, m, l][row]
+constexpr int CHUNK_PART_LD = CHUNK_DIM + 4;                     // a row's o, m, l
+constexpr int CHUNK_PART_FLOATS = CHUNK_PART_LD * CHUNK_PART_ROWS;
 
+// What CTA c leaves behind: at most one block that it began and others finish (partials in slot 2c + 1), and one
+// that it only went on with (slot 2c).
 struct ChunkMeta {
-  int state;  // 1: this CTA began a block that others finish; 2: a wait gave up
-  int row0, ntok, head, nt, pos0;
-  long long base, total;
+  int state;  // 1: it began such a block; 2: a wait gave up
+  int row0, ntok, head, pos0;
+  int went_on;  // 1: it went on with the block of the CTAs before it; 2: and finished it
 };
 __host__ __device__ constexpr long long chunk_meta_bytes(int grid) { return (grid * 64ll + 255) / 256 * 256; }
 __host__ __device__ constexpr long long chunk_ws_bytes(int grid) {
@@ -256,6 +259,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -364,7 +372,6 @@ struct ChunkBlock {
   int head, slot;
   int t0, nt, tiles;   // key tiles [t0, t0 + nt) of the block's `tiles`
   int nt0;             // of two row tiles: how many of the nt the first one sees
-  long long base;
   int pages[16];       // the first pages of the range
 };
 constexpr int CHUNK_BLOCKS = 3;
@@ -516,12 +523,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     return B.block[n % CHUNK_BLOCKS].more;
   };
   ChunkMeta* meta = reinterpret_cast<ChunkMeta*>(a.ws + static_cast<size_t>(cta) * 64);
-  if (tid == 128) meta->state = 0;  // (the thread that may set it to 1)
+  if (tid == 128) meta->state = meta->went_on = 0;  // (the thread that may set them)
 
   if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");  // 256 x 208 + 128 x 88 = the launch's 384 x 168
     // ================================================================ softmax and output
     const int grp = (warp >> 2) - 1, row = (warp & 3) * 32 + lane;
+    const int row_tok = row / group, row_head = row % group;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + grp * 128 + lanes, t_o = tmem + 256 + grp * 128 + lanes;
     uint32_t n_tile = 0, n_out = 0, n_merge = 0;  // this group's tiles and blocks, and merges, so far
@@ -529,10 +537,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const ChunkBlock& d = B.block[n_unit % CHUNK_BLOCKS];
       const int nt = d.nt;
       const bool pair = d.ntok > T_tok;
-      const bool valid = row < T_tok * group && (pair ? grp * T_tok : 0) + row / group < d.ntok;
+      const bool valid = row_tok < T_tok && (pair ? grp * T_tok : 0) + row_tok < d.ntok;
       const bool live = __any_sync(0xffffffffu, valid);
       // the last key that the row sees, counted from the range's first
-      const int limit = valid ? d.pos0 + (pair ? grp * T_tok : 0) + row / group - d.t0 * CHUNK_KT : -1;
+      const int limit = valid ? d.pos0 + (pair ? grp * T_tok : 0) + row_tok - d.t0 * CHUNK_KT : -1;
       const int step = pair ? 1 : 2, first = pair ? 0 : grp, count = pair && grp == 0 ? d.nt0 : nt;
       float m = -INFINITY, l = 0.0f;
       for (int j = first; j < count; j += step, ++n_tile) {
@@ -642,64 +650,104 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
       }
       const bool whole = nt == d.tiles;
-      const int tok = (pair ? grp * T_tok : 0) + row / group, pos = d.pos0 + tok;
+      const int tok = (pair ? grp * T_tok : 0) + row_tok, pos = d.pos0 + tok;
       const bool seen = pos >= 0;
-      const int out_row = d.row0 + tok, qhead = d.head * group + row % group;
+      const int out_row = d.row0 + tok, qhead = d.head * group + row_head;
       const int prow = (pair ? grp * 128 : 0) + row;
       float* part = chunk_part(a, grid, d.t0 == 0 ? 2 * cta + 1 : 2 * cta);
       float bad = 0.0f;
       if (live) {
-        const float inv = whole ? (seen ? 1.0f / l : 0.0f) : 1.0f;
-        const float g0 = f0 * inv, g1 = f1 * inv;
-        uint8_t* stage = sm_out + (warp - 4) * CHUNK_OUT_BYTES;
+        const float inv = whole ? 1.0f / l : 1.0f;
+        const float g0 = seen ? f0 * inv : 0.0f, g1 = seen ? f1 * inv : 0.0f;
+        const uint64_t g0x2 = pack2(g0, g0), g1x2 = pack2(g1, g1);
         const unsigned rows_valid = __ballot_sync(0xffffffffu, valid);
         const bool any1 = __any_sync(0xffffffffu, has1);
+        // In nearly every block all rows saw keys in what is joined; where one did not, O may hold anything there.
+        const bool plain = !__any_sync(0xffffffffu, valid && !(seen && has0 && (has1 || !any1)));
+        uint8_t* stage = sm_out + (warp - 4) * CHUNK_OUT_BYTES;
+        uint64_t bad2 = 0;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          float o[32], o1[32];
+          float o[32];
           tmem_ld_x32(t_o + c * 32, o);
-          if (any1) tmem_ld_x32(t_o + 128 + c * 32, o1);
-          tmem_wait_ld();
+          if (any1) {
+            float o1[32];
+            tmem_ld_x32(t_o + 128 + c * 32, o1);
+            tmem_wait_ld();
+            if (!plain) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            float v = has0 ? o[x] * g0 : 0.0f;
-            if (has1) v = fmaf(o1[x], g1, v);
-            v = seen ? v : 0.0f;
-            bad = fmaf(v, 0.0f, bad);  // NaN once a value is not finite
-            o[x] = v;
-          }
-          if (!whole) {
-            if (valid)
+              for (int x = 0; x < 32; ++x) {
+                o[x] = has0 ? o[x] : 0.0f;
+                o1[x] = has1 ? o1[x] : 0.0f;
+              }
+            }
 #pragma unroll
-              for (int x = 0; x < 32; ++x) part[(c * 32 + x) * CHUNK_PART_ROWS + prow] = o[x];
-            continue;
-          }
-          // through shared memory, so that a store covers whole sectors: 32 dims of 8 rows
+            for (int x = 0; x < 32; x += 2) {
+              const uint64_t v = fma2(pack2(o1[x], o1[x + 1]), g1x2, mul2(pack2(o[x], o[x + 1]), g0x2));
+              bad2 = fma2(v, 0, bad2);  // NaN once a value is not finite
+              unpack2(v, o[x], o[x + 1]);
+            }
+          } else {
+            tmem_wait_ld();
+            if (!plain) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint4 v;
-            v.x = TT::from_f32(o[8 * x], o[8 * x + 1]);
-            v.y = TT::from_f32(o[8 * x + 2], o[8 * x + 3]);
-            v.z = TT::from_f32(o[8 * x + 4], o[8 * x + 5]);
-            v.w = TT::from_f32(o[8 * x + 6], o[8 * x + 7]);
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((x ^ (lane >> 1 & 3)) * 16)) = v;
-          }
-          __syncwarp();
-          for (int y = 0; y < 4; ++y) {
-            const int r = y * 8 + (lane >> 2);
-            if (!(rows_valid >> (y * 8) & 255)) continue;
-            const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
-            if (rows_valid >> r & 1) {
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) * 16));
-              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
-                                        c * 32 + (lane & 3) * 8) = v;
+              for (int x = 0; x < 32; ++x) o[x] = seen && has0 ? o[x] : 0.0f;
+            }
+#pragma unroll
+            for (int x = 0; x < 32; x += 2) {
+              const uint64_t v = mul2(pack2(o[x], o[x + 1]), g0x2);
+              bad2 = fma2(v, 0, bad2);
+              unpack2(v, o[x], o[x + 1]);
             }
           }
-          __syncwarp();
+          if (!seen) {  // zeros, whatever stands there
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = 0.0f;
+          }
+          // Through shared memory, 64 bytes a row, so that a store covers whole sectors of 8 rows: 32 dims in the
+          // output's type, or the partial's in two halves.
+          const int steps = whole ? 1 : 2;
+          for (int h = 0; h < steps; ++h) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint4 v;
+              if (whole) {
+                v.x = TT::from_f32(o[8 * x], o[8 * x + 1]);
+                v.y = TT::from_f32(o[8 * x + 2], o[8 * x + 3]);
+                v.z = TT::from_f32(o[8 * x + 4], o[8 * x + 5]);
+                v.w = TT::from_f32(o[8 * x + 6], o[8 * x + 7]);
+              } else {
+                v.x = __float_as_uint(h ? o[16 + 4 * x] : o[4 * x]);
+                v.y = __float_as_uint(h ? o[17 + 4 * x] : o[4 * x + 1]);
+                v.z = __float_as_uint(h ? o[18 + 4 * x] : o[4 * x + 2]);
+                v.w = __float_as_uint(h ? o[19 + 4 * x] : o[4 * x + 3]);
+              }
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((x ^ (lane >> 1 & 3)) * 16)) = v;
+            }
+            __syncwarp();
+#pragma unroll 1
+            for (int y = 0; y < 4; ++y) {
+              const int r = y * 8 + (lane >> 2);
+              if (!(rows_valid >> (y * 8) & 255)) continue;
+              const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
+              if (rows_valid >> r & 1) {
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) * 16));
+                if (whole)
+                  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
+                                            c * 32 + (lane & 3) * 8) = v;
+                else
+                  *reinterpret_cast<uint4*>(part + (prow - lane + r) * CHUNK_PART_LD + c * 32 + h * 16 + (lane & 3) * 4) = v;
+              }
+            }
+            __syncwarp();
+          }
         }
+        float b0, b1;
+        unpack2(bad2, b0, b1);
+        bad = seen ? b0 + b1 : 0.0f;
         if (valid && !whole) {
-          part[CHUNK_DIM * CHUNK_PART_ROWS + prow] = m;
-          part[(CHUNK_DIM + 1) * CHUNK_PART_ROWS + prow] = l;
+          part[prow * CHUNK_PART_LD + CHUNK_DIM] = m;
+          part[prow * CHUNK_PART_LD + CHUNK_DIM + 1] = l;
         }
       }
       tc_fence_before();
@@ -724,25 +772,23 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(r_row) * a.out_ld + r_head * CHUNK_DIM +
                                     lane * 4) = v;
         } else {
-          part[(lane * 4) * CHUNK_PART_ROWS + r_prow] = o.x;
-          part[(lane * 4 + 1) * CHUNK_PART_ROWS + r_prow] = o.y;
-          part[(lane * 4 + 2) * CHUNK_PART_ROWS + r_prow] = o.z;
-          part[(lane * 4 + 3) * CHUNK_PART_ROWS + r_prow] = o.w;
+          *reinterpret_cast<float4*>(part + r_prow * CHUNK_PART_LD + lane * 4) = o;
           if (lane == 0) {
-            part[CHUNK_DIM * CHUNK_PART_ROWS + r_prow] = rm;
-            part[(CHUNK_DIM + 1) * CHUNK_PART_ROWS + r_prow] = rl;
+            part[r_prow * CHUNK_PART_LD + CHUNK_DIM] = rm;
+            part[r_prow * CHUNK_PART_LD + CHUNK_DIM + 1] = rl;
           }
         }
       }
-      if (!whole && d.t0 == 0 && grp == 0 && row == 0) {
-        meta->row0 = d.row0;
-        meta->ntok = d.ntok;
-        meta->head = d.head;
-        meta->nt = d.tiles;
-        meta->pos0 = d.pos0;
-        meta->base = d.base;
-        meta->total = total;
-        meta->state = 1;
+      if (!whole && grp == 0 && row == 0) {
+        if (d.t0 == 0) {
+          meta->row0 = d.row0;
+          meta->ntok = d.ntok;
+          meta->head = d.head;
+          meta->pos0 = d.pos0;
+          meta->state = 1;
+        } else {
+          meta->went_on = d.t0 + nt == d.tiles ? 2 : 1;
+        }
       }
     }
   softmax_out:;
@@ -950,7 +996,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           d.nt = w.t1 - w.t0;
           d.tiles = w.nt;
           d.nt0 = min(max((pos0 + T_tok + CHUNK_KT - 1) / CHUNK_KT - w.t0, 0), d.nt);  // (0 where nothing is seen)
-          d.base = w.base;
         }
       }
       __syncwarp();
@@ -981,53 +1026,59 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-// Joins the partials of the block that CTA blockIdx.x began and others went on with; blockIdx.y takes
-// 32 rows of it, a thread one row and 16 dims.
+// Joins the partials of the block that CTA blockIdx.x began and the CTAs behind it went on with: a warp a row, a lane four
+// dims.  Bound by its chain of loads (what was left behind, then m and l of all parts at once, then o).
+constexpr int CHUNK_COMBINE_WARPS = 8;
 template <bool BF16>
-__global__ void __launch_bounds__(256) attention_chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int grid) {
+__global__ void __launch_bounds__(CHUNK_COMBINE_WARPS * 32) attention_chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int grid) {
   using TT = ChunkType<BF16>;
   using T = typename TT::T;
+  const int lane = threadIdx.x & 31, c0 = blockIdx.x;
+  const int prow = blockIdx.y * CHUNK_COMBINE_WARPS + (threadIdx.x >> 5);
+  const int group = a.group, T_tok = a.tile_tokens;
+  const int tok = (prow >> 7) * T_tok + (prow & 127) / group, head_of = (prow & 127) % group;
   griddep_wait();
   griddep_launch_dependents();
-  const ChunkMeta* meta = reinterpret_cast<const ChunkMeta*>(a.ws + static_cast<size_t>(blockIdx.x) * 64);
-  if (meta->state != 1) return;
-  const int group = a.group, T_tok = a.tile_tokens;
-  const int prow = blockIdx.y * 32 + (threadIdx.x & 31), col = (threadIdx.x >> 5) * 16;
-  const int tok = (prow >> 7) * T_tok + (prow & 127) / group, head = meta->head * group + (prow & 127) % group;
-  if ((prow & 127) >= T_tok * group || tok >= meta->ntok) return;
-  const int nt = meta->nt;
-  const long long base = meta->base, total = meta->total;
-  float top = -INFINITY;
-  for (int pass = 0; pass < 2; ++pass) {
-    float l = 0.0f, o[16] = {};
-    for (int c = blockIdx.x, end = 0; end < nt && c < grid; ++c) {
-      const int t0 = chunk_cut(chunk_bound(total, c, grid), base, nt), t1 = chunk_cut(chunk_bound(total, c + 1, grid), base, nt);
-      end = t1;
-      if (t1 <= t0) continue;
-      const float* part = chunk_part(a, grid, c == static_cast<int>(blockIdx.x) ? 2 * c + 1 : 2 * c) + prow;
-      const float m = part[CHUNK_DIM * CHUNK_PART_ROWS];
-      if (pass == 0) {
-        top = fmaxf(top, m);
-      } else if (m != -INFINITY) {
-        const float f = ex2(m - top);
-        l += part[(CHUNK_DIM + 1) * CHUNK_PART_ROWS] * f;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) o[x] += part[(col + x) * CHUNK_PART_ROWS] * f;
-      }
-    }
-    if (pass == 0) continue;
-    const float inv = meta->pos0 + tok < 0 ? 0.0f : 1.0f / l;
-    T* out = static_cast<T*>(a.out) + static_cast<size_t>(meta->row0 + tok) * a.out_ld + head * CHUNK_DIM + col;
-#pragma unroll
-    for (int x = 0; x < 16; x += 8) {
-      uint4 v;
-      v.x = TT::from_f32(o[x] * inv, o[x + 1] * inv);
-      v.y = TT::from_f32(o[x + 2] * inv, o[x + 3] * inv);
-      v.z = TT::from_f32(o[x + 4] * inv, o[x + 5] * inv);
-      v.w = TT::from_f32(o[x + 6] * inv, o[x + 7] * inv);
-      *reinterpret_cast<uint4*>(out + x) = v;
-    }
+  auto line = [&](int c) { return reinterpret_cast<const ChunkMeta*>(a.ws + static_cast<size_t>(c) * 64); };
+  const ChunkMeta mine = *line(c0);
+  int next = c0 + 1 + lane < grid ? line(c0 + 1 + lane)->went_on : 0;
+  if (mine.state != 1 || (prow & 127) >= T_tok * group || tok >= mine.ntok) return;
+  // parts: this CTA's, then those of the CTAs that went on, up to the one that finished; 32 CTAs at a time
+  const float* first = chunk_part(a, grid, 2 * c0 + 1) + prow * CHUNK_PART_LD;
+  float top = first[CHUNK_DIM], sum = first[CHUNK_DIM + 1];
+  float4 o = *reinterpret_cast<const float4*>(first + lane * 4);
+  if (top == -INFINITY) {
+    sum = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
+  for (int c1 = c0 + 1; c1 < grid; c1 += 32) {
+    const unsigned ends = __ballot_sync(0xffffffffu, next == 2);
+    unsigned on = __ballot_sync(0xffffffffu, next != 0);
+    if (ends) on &= (2u << (__ffs(ends) - 1)) - 1;
+    const float* part = chunk_part(a, grid, 2 * min(c1 + lane, grid - 1)) + prow * CHUNK_PART_LD;
+    const float2 ml = on >> lane & 1 ? *reinterpret_cast<const float2*>(part + CHUNK_DIM) : make_float2(-INFINITY, 0.0f);
+    for (; on; on &= on - 1) {
+      const int i = __ffs(on) - 1;
+      const float m = __shfl_sync(0xffffffffu, ml.x, i), l = __shfl_sync(0xffffffffu, ml.y, i);
+      const float4 v = *reinterpret_cast<const float4*>(chunk_part(a, grid, 2 * (c1 + i)) + prow * CHUNK_PART_LD + lane * 4);
+      if (m == -INFINITY) continue;  // it saw nothing of this row's: its o may be anything
+      const float t = fmaxf(top, m), f0 = top == -INFINITY ? 0.0f : ex2(top - t), f1 = ex2(m - t);
+      sum = sum * f0 + l * f1;
+      o.x = o.x * f0 + v.x * f1;
+      o.y = o.y * f0 + v.y * f1;
+      o.z = o.z * f0 + v.z * f1;
+      o.w = o.w * f0 + v.w * f1;
+      top = t;
+    }
+    if (ends) break;
+    next = c1 + 32 + lane < grid ? line(c1 + 32 + lane)->went_on : 0;
+  }
+  const float inv = mine.pos0 + tok < 0 ? 0.0f : 1.0f / sum;
+  uint2 v;
+  v.x = TT::from_f32(o.x * inv, o.y * inv);
+  v.y = TT::from_f32(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(mine.row0 + tok) * a.out_ld +
+                            (mine.head * group + head_of) * CHUNK_DIM + lane * 4) = v;
 }
 
 }  // namespace qasr

@@ -284,10 +284,11 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
   e = bf ? launch_k(attention_chunk_kernel<true>, dim3(grid), dim3(CHUNK_THREADS), CHUNK_SMEM, st, true, q_big, q_small, kv_map, a)
          : launch_k(attention_chunk_kernel<false>, dim3(grid), dim3(CHUNK_THREADS), CHUNK_SMEM, st, true, q_big, q_small, kv_map, a);
   if (e != cudaSuccess) return op_cuda(err, errlen, e, "chunk attention launch");
-  // 32 of a block's packed rows each; no block has more rows than the call
-  const dim3 cgrid(grid, rows <= chunk_tile_tokens(group) ? (rows * group + 31) / 32 : CHUNK_PART_ROWS / 32);
-  e = bf ? launch_k(attention_chunk_combine_kernel<true>, cgrid, dim3(256), 0, st, true, a, grid)
-         : launch_k(attention_chunk_combine_kernel<false>, cgrid, dim3(256), 0, st, true, a, grid);
+  // a warp per packed row of a block, of which none has more than the call
+  const int packed = rows <= chunk_tile_tokens(group) ? rows * group : CHUNK_PART_ROWS;
+  const dim3 cgrid(grid, (packed + CHUNK_COMBINE_WARPS - 1) / CHUNK_COMBINE_WARPS);
+  e = bf ? launch_k(attention_chunk_combine_kernel<true>, cgrid, dim3(CHUNK_COMBINE_WARPS * 32), 0, st, true, a, grid)
+         : launch_k(attention_chunk_combine_kernel<false>, cgrid, dim3(CHUNK_COMBINE_WARPS * 32), 0, st, true, a, grid);
   return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "chunk attention combine launch");
 }
 
