@@ -162,54 +162,88 @@ __device__ __forceinline__ long long chunk_bound(long long total, int c, int gri
     return static_cast<uint32_t>(total) * static_cast<uint32_t>(c) / static_cast<uint32_t>(grid);
   return total * c / grid;
 }
-// The first key tile behind cut x of a block that starts at `base`.
-__device__ __forceinline__ int chunk_cut(long long x, long long base, int nt) {
-  const long long t = x - base - CHUNK_BLOCK_COST;
+// The first key tile behind a cut `x` cost units into a block.
+__device__ __forceinline__ int chunk_cut(int x, int nt) {
+  const int t = x - CHUNK_BLOCK_COST;
   if (t >= nt) return nt;
   if (t <= CHUNK_SNAP) return 0;
-  return nt - t <= CHUNK_SNAP ? nt : static_cast<int>(t);
+  return nt - t <= CHUNK_SNAP ? nt : t;
 }
 
 struct ChunkWalk {
   int i, g, k, nb, nt, t0, t1;
-  long long base, lo, hi;
+  int at, hi;  // the block's and the range's end, counted from the range's start
   ChunkSeq s;
 };
-// Fit the walk's block to the CTA's range; false past its end.  Blocks without a tile in the range are passed over.
+// On to the next block; false past the last.
+__device__ __forceinline__ bool chunk_step(const ChunkArgs& a, ChunkWalk& w, int bt) {
+  w.at += w.nt + CHUNK_BLOCK_COST;
+  if (++w.k < w.nb) return true;
+  w.k = 0;
+  if (++w.g < a.nkv) return true;
+  w.g = 0;
+  do {
+    if (++w.i >= a.n_seqs) return false;
+    w.s = chunk_seq(a, w.i);
+  } while (w.s.n == 0);
+  w.nb = chunk_blocks(w.s.n, bt);
+  return true;
+}
+// Fit the walk's block to the CTA's range, passing over blocks without a tile in it; false past its end.
 __device__ __forceinline__ bool chunk_fit(const ChunkArgs& a, ChunkWalk& w, int bt) {
-  while (w.i < a.n_seqs && w.base < w.hi) {
+  while (w.at < w.hi) {
     w.nt = chunk_tiles(w.s, w.k, bt);
-    w.t0 = chunk_cut(w.lo, w.base, w.nt);
-    w.t1 = chunk_cut(w.hi, w.base, w.nt);
+    w.t0 = chunk_cut(-w.at, w.nt);
+    w.t1 = chunk_cut(w.hi - w.at, w.nt);
     if (w.t1 > w.t0) return true;
-    w.base += w.nt + CHUNK_BLOCK_COST;
-    if (++w.k == w.nb) {
-      w.k = 0;
-      if (++w.g == a.nkv) {
-        w.g = 0;
-        do {
-          if (++w.i >= a.n_seqs) return false;
-          w.s = chunk_seq(a, w.i);
-        } while (w.s.n == 0);
-        w.nb = chunk_blocks(w.s.n, bt);
-      }
-    }
+    if (!chunk_step(a, w, bt)) return false;
   }
   return false;
 }
-__device__ __forceinline__ bool chunk_next(const ChunkArgs& a, ChunkWalk& w, int bt) {
-  w.base += w.nt + CHUNK_BLOCK_COST;
-  if (++w.k == w.nb) {
-    w.k = 0;
-    if (++w.g == a.nkv) {
-      w.g = 0;
-      do {
-        if (++w.i >= a.n_seqs) return false;
-        w.s = chunk_seq(a, w.i);
-      } while (w.s.n == 0);
-      w.nb = chunk_blocks(w.s.n, bt);
-    }
+
+// The first block of CTA `cta`'s range, found by one warp: a lane sums the costs of n_seqs / 32 requests, a scan places them.
+// (All the CTA's threads would sum 512 requests sooner, but two block-wide steps cost more than that gains.)
+__device__ __forceinline__ bool chunk_begin(const ChunkArgs& a, ChunkWalk& w, int cta, int grid, int bt) {
+  const int lane = threadIdx.x & 31, per = (a.n_seqs + 31) / 32, i0 = min(lane * per, a.n_seqs), i1 = min(i0 + per, a.n_seqs);
+  long long mine = 0;
+  ChunkSeq s{};
+  for (int i = i0; i < i1; ++i) {
+    s = chunk_seq(a, i);
+    mine += chunk_head_cost(s, bt) * a.nkv;
   }
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  const long long total = __shfl_sync(0xffffffffu, incl, 31);
+  const long long lo = chunk_bound(total, cta, grid), hi = chunk_bound(total, cta + 1, grid);
+  if (lo >= hi) return false;
+  const int src = __ffs(__ballot_sync(0xffffffffu, lo < incl)) - 1;
+  w.hi = static_cast<int>(min(hi - lo, 0x7fffffffll));
+  w.i = __shfl_sync(0xffffffffu, i0, src);
+  long long at = __shfl_sync(0xffffffffu, incl - mine, src) - lo;  // <= 0
+  w.s.row0 = __shfl_sync(0xffffffffu, s.row0, src);
+  w.s.n = __shfl_sync(0xffffffffu, s.n, src);
+  w.s.len = __shfl_sync(0xffffffffu, s.len, src);
+  w.s.slot = __shfl_sync(0xffffffffu, s.slot, src);
+  long long head = 0;
+  while (true) {  // the lane's request, its head, its block
+    if (per > 1) w.s = chunk_seq(a, w.i);
+    head = chunk_head_cost(w.s, bt);
+    if (at + head * a.nkv > 0) break;
+    at += head * a.nkv;
+    ++w.i;
+  }
+  for (w.g = 0; at + head <= 0; ++w.g) at += head;
+  w.nb = chunk_blocks(w.s.n, bt);
+  for (w.k = 0;; ++w.k) {
+    const int cost = chunk_tiles(w.s, w.k, bt) + CHUNK_BLOCK_COST;
+    if (at + cost > 0) break;
+    at += cost;
+  }
+  w.at = static_cast<int>(at);
   return chunk_fit(a, w, bt);
 }
 
@@ -387,11 +421,6 @@ struct ChunkBars {
   ChunkBlock block[CHUNK_BLOCKS];
   uint32_t tmem;
   int abort_flag;
-  // the range's first block
-  int i, g, k, any;
-  ChunkSeq seq;
-  long long base;
-  long long scan[CHUNK_THREADS / 32];
 };
 static_assert(sizeof(ChunkBars) <= 1024, "ChunkBars sits in the last KB of the shared memory");
 
@@ -438,7 +467,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&B.block_free[i], 11);
     }
     B.abort_flag = 0;
-    B.any = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -453,58 +481,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   griddep_wait();
   griddep_launch_dependents();
 
-  // ---- the call's total cost and the first block of this CTA's range
-  const int per = (a.n_seqs + CHUNK_THREADS - 1) / CHUNK_THREADS;
-  const int i0 = min(tid * per, a.n_seqs), i1 = min(i0 + per, a.n_seqs);
-  long long mine = 0;
-  ChunkSeq s{};
-  long long head_cost = 0;  // (of the thread's only request, in most calls)
-  for (int i = i0; i < i1; ++i) {
-    s = chunk_seq(a, i);
-    head_cost = chunk_head_cost(s, bt);
-    mine += head_cost * a.nkv;
-  }
-  long long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) B.scan[warp] = incl;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  long long total = 0;
-  for (int i = 0; i < CHUNK_THREADS / 32; ++i) {
-    if (i < warp) incl += B.scan[i];
-    total += B.scan[i];
-  }
-  const long long lo = chunk_bound(total, cta, grid), hi = chunk_bound(total, cta + 1, grid);
-  if (lo < hi && incl - mine <= lo && lo < incl) {
-    long long base = incl - mine;
-    int i = i0;
-    while (per > 1) {
-      s = chunk_seq(a, i);
-      head_cost = chunk_head_cost(s, bt);
-      if (lo < base + head_cost * a.nkv) break;
-      base += head_cost * a.nkv;
-      ++i;
-    }
-    int g = 0;
-    for (; lo >= base + head_cost; ++g) base += head_cost;
-    int k = 0;
-    while (lo >= base + chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST) {
-      base += chunk_tiles(s, k, bt) + CHUNK_BLOCK_COST;
-      ++k;
-    }
-    B.i = i;
-    B.g = g;
-    B.k = k;
-    B.base = base;
-    B.seq = s;
-    B.any = 1;
-  }
-  __syncthreads();
   const uint32_t tmem = B.tmem;
   volatile int* abort_flag = &B.abort_flag;
   // block n of the range: 1 there, 0 the range is over, -1 a wait gave up
@@ -666,9 +645,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const bool plain = !__any_sync(0xffffffffu, valid && !(seen && has0 && (has1 || !any1)));
         uint8_t* stage = sm_out + (warp - 4) * CHUNK_OUT_BYTES;
         uint64_t bad2 = 0;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
+        // dims 32c .. 32c + 31 of this thread's row
+        auto fetch = [&](int c, float (&o)[32]) {
           tmem_ld_x32(t_o + c * 32, o);
           if (any1) {
             float o1[32];
@@ -691,7 +669,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             tmem_wait_ld();
             if (!plain) {
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = seen && has0 ? o[x] : 0.0f;
+              for (int x = 0; x < 32; ++x) o[x] = has0 ? o[x] : 0.0f;
             }
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
@@ -700,54 +678,92 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               unpack2(v, o[x], o[x + 1]);
             }
           }
-          if (!seen) {  // zeros, whatever stands there
+          if (!plain) {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = 0.0f;
+            for (int x = 0; x < 32; ++x) o[x] = seen ? o[x] : 0.0f;  // zeros, whatever stands there
           }
+        };
+        auto pack8 = [&](const float* o) {
+          uint4 v;
+          v.x = TT::from_f32(o[0], o[1]);
+          v.y = TT::from_f32(o[2], o[3]);
+          v.z = TT::from_f32(o[4], o[5]);
+          v.w = TT::from_f32(o[6], o[7]);
+          return v;
+        };
+        float* my_part = part + prow * CHUNK_PART_LD;
+        if (__popc(rows_valid) <= 4) {  // as in a decode step: a row's stores straight out of its thread are the shorter way
+          T* to = static_cast<T*>(a.out) + static_cast<size_t>(out_row) * a.out_ld + qhead * CHUNK_DIM;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            fetch(c, o);
+            if (!valid) continue;
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+              if (whole) {
+                *reinterpret_cast<uint4*>(to + c * 32 + x) = pack8(o + x);
+              } else {
+                *reinterpret_cast<float4*>(my_part + c * 32 + x) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                *reinterpret_cast<float4*>(my_part + c * 32 + x + 4) = make_float4(o[x + 4], o[x + 5], o[x + 6], o[x + 7]);
+              }
+            }
+          }
+        } else {
           // Through shared memory, 64 bytes a row, so that a store covers whole sectors of 8 rows: 32 dims in the
           // output's type, or the partial's in two halves.
-          const int steps = whole ? 1 : 2;
-          for (int h = 0; h < steps; ++h) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint4 v;
-              if (whole) {
-                v.x = TT::from_f32(o[8 * x], o[8 * x + 1]);
-                v.y = TT::from_f32(o[8 * x + 2], o[8 * x + 3]);
-                v.z = TT::from_f32(o[8 * x + 4], o[8 * x + 5]);
-                v.w = TT::from_f32(o[8 * x + 6], o[8 * x + 7]);
-              } else {
-                v.x = __float_as_uint(h ? o[16 + 4 * x] : o[4 * x]);
-                v.y = __float_as_uint(h ? o[17 + 4 * x] : o[4 * x + 1]);
-                v.z = __float_as_uint(h ? o[18 + 4 * x] : o[4 * x + 2]);
-                v.w = __float_as_uint(h ? o[19 + 4 * x] : o[4 * x + 3]);
-              }
-              *reinterpret_cast<uint4*>(stage + lane * 64 + ((x ^ (lane >> 1 & 3)) * 16)) = v;
-            }
+          uint4* put = reinterpret_cast<uint4*>(stage + lane * 64);
+          const int put_x = lane >> 1 & 3;
+          auto send = [&](auto to) {  // `to`(r, lane's 16-byte chunk) stores row r's chunk lane & 3
             __syncwarp();
 #pragma unroll 1
             for (int y = 0; y < 4; ++y) {
               const int r = y * 8 + (lane >> 2);
-              if (!(rows_valid >> (y * 8) & 255)) continue;
-              const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
-              if (rows_valid >> r & 1) {
-                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) * 16));
-                if (whole)
-                  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
-                                            c * 32 + (lane & 3) * 8) = v;
-                else
-                  *reinterpret_cast<uint4*>(part + (prow - lane + r) * CHUNK_PART_LD + c * 32 + h * 16 + (lane & 3) * 4) = v;
-              }
+              to(r, *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) * 16)));
             }
             __syncwarp();
+          };
+          if (whole) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float o[32];
+              fetch(c, o);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) put[x ^ put_x] = pack8(o + 8 * x);
+              send([&](int r, uint4 v) {
+                const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
+                if (rows_valid >> r & 1)
+                  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
+                                            c * 32 + (lane & 3) * 8) = v;
+              });
+            }
+          } else {
+            float* warp_part = my_part - lane * CHUNK_PART_LD;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float o[32];
+              fetch(c, o);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float* f = o + h * 16 + 4 * x;
+                  put[x ^ put_x] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+                }
+                send([&](int r, uint4 v) {
+                  if (rows_valid >> r & 1)
+                    *reinterpret_cast<uint4*>(warp_part + r * CHUNK_PART_LD + c * 32 + h * 16 + (lane & 3) * 4) = v;
+                });
+              }
+            }
           }
         }
         float b0, b1;
         unpack2(bad2, b0, b1);
         bad = seen ? b0 + b1 : 0.0f;
         if (valid && !whole) {
-          part[prow * CHUNK_PART_LD + CHUNK_DIM] = m;
-          part[prow * CHUNK_PART_LD + CHUNK_DIM + 1] = l;
+          my_part[CHUNK_DIM] = m;
+          my_part[CHUNK_DIM + 1] = l;
         }
       }
       tc_fence_before();
@@ -961,18 +977,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ================================================================ the walk
     ChunkWalk w;
-    bool more = B.any != 0;
-    if (more) {
-      w.i = B.i;
-      w.g = B.g;
-      w.k = B.k;
-      w.base = B.base;
-      w.lo = lo;
-      w.hi = hi;
-      w.s = B.seq;
-      w.nb = chunk_blocks(w.s.n, bt);
-      more = chunk_fit(a, w, bt);
-    }
+    bool more = chunk_begin(a, w, cta, grid, bt);
     // Block n is handed on while block n - 1 is worked at; then comes the clearing for block n - 1, so nothing that a
     // block waits for ever stands behind a wait for that block.
     uint32_t n_clear = 0;
@@ -1016,7 +1021,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       }
       if (!more) break;
       clear_before = clear;
-      more = chunk_next(a, w, bt);
+      more = chunk_step(a, w, bt) && chunk_fit(a, w, bt);
     }
   }
   tc_fence_before();
