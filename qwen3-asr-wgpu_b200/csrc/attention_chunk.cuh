@@ -25,8 +25,9 @@
 // waits hold up the other; warp 2's copies Q and the pages.  Warp 3 walks the schedule and hands the others one block
 // after the other through shared memory, which keeps the walk out of their registers, and clears V rows for
 // warp 1.  Warps 4-7 and 8-11 are two softmax groups, one per row tile.  A block of one row tile only (a
-// decode step, a short chunk) gives its even key tiles to the first group and the odd ones to the second; the first
-// then joins both results, which stand in the same tensor memory lanes.  So both always have work.
+// decode step, a short chunk) gives its even key tiles to the first group and the odd ones to the second; both
+// results stand in the same tensor memory lanes, and each group then joins them for half of the dims.  So both always have
+// work.
 //
 // Work split: every (request, kv head, block) costs its key tiles plus CHUNK_BLOCK_COST; the costs of the whole call,
 // laid end to end, are cut into one equal range per CTA.  A block that a cut goes through leaves f32
@@ -75,7 +76,7 @@ constexpr int CHUNK_HALF_BYTES = CHUNK_KT * 128;  // the rows' first or second 6
 constexpr int CHUNK_Q_TILE = 128 * CHUNK_DIM * 2, CHUNK_Q_HALF = CHUNK_Q_TILE / 2;
 constexpr int CHUNK_Q_BYTES = 2 * CHUNK_Q_TILE;
 constexpr int CHUNK_OUT_BYTES = 32 * 64;           // per softmax warp: a quarter of its rows' output
-constexpr int CHUNK_SMEM = 1024 + CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 2048;
+constexpr int CHUNK_SMEM = CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 3072;
 constexpr int CHUNK_BLOCK_COST = 2;               // a block's Q copy, first and last steps, in key tiles
 constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
@@ -201,47 +202,75 @@ __device__ __forceinline__ bool chunk_fit(const ChunkArgs& a, ChunkWalk& w, int 
   return false;
 }
 
-// The first block of CTA `cta`'s range, found by one warp: a lane sums the costs of n_seqs / 32 requests, a scan places them.
-// (All the CTA's threads would sum 512 requests sooner, but two block-wide steps cost more than that gains.)
+// The first block of CTA `cta`'s range, found by one warp.  The requests are cut into 32 runs, one a lane; 32 requests of a
+// run are read at a time, and a scan over the runs' costs, then one inside the run that holds the start, finds the request.
 __device__ __forceinline__ bool chunk_begin(const ChunkArgs& a, ChunkWalk& w, int cta, int grid, int bt) {
-  const int lane = threadIdx.x & 31, per = (a.n_seqs + 31) / 32, i0 = min(lane * per, a.n_seqs), i1 = min(i0 + per, a.n_seqs);
-  long long mine = 0;
-  ChunkSeq s{};
-  for (int i = i0; i < i1; ++i) {
+  const int lane = threadIdx.x & 31, steps = (a.n_seqs + 1023) / 1024, runs = (a.n_seqs + steps * 32 - 1) / (steps * 32);
+  auto cost_of = [&](ChunkSeq& s, int i) {
+    if (i >= a.n_seqs) return 0ll;
     s = chunk_seq(a, i);
-    mine += chunk_head_cost(s, bt) * a.nkv;
-  }
-  long long incl = mine;
+    return chunk_head_cost(s, bt) * a.nkv;
+  };
+  auto scan = [&](long long v) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  ChunkSeq s{};
+  long long cost = 0, mine = 0;
+  const bool one = runs == 1 && steps == 1;  // one read is all
+  if (one) cost = cost_of(s, lane);
+  for (int r = 0; !one && r < runs; r += 4) {  // four runs' reads at a time
+    long long sum[4] = {};
+    for (int x = 0; x < steps; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) sum[y] += cost_of(s, ((r + y) * steps + x) * 32 + lane);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], o);
+      if (lane == r + y) mine = sum[y];
+    }
   }
-  const long long total = __shfl_sync(0xffffffffu, incl, 31);
+  long long total, at = 0;  // `at`: the cost before the run, then before the request
+  int run = 0;
+  long long incl = scan(one ? cost : mine);
+  total = __shfl_sync(0xffffffffu, incl, 31);
   const long long lo = chunk_bound(total, cta, grid), hi = chunk_bound(total, cta + 1, grid);
   if (lo >= hi) return false;
-  const int src = __ffs(__ballot_sync(0xffffffffu, lo < incl)) - 1;
+  int src = __ffs(__ballot_sync(0xffffffffu, lo < incl)) - 1, i = 0;
+  if (!one) {
+    run = src;
+    at = __shfl_sync(0xffffffffu, incl - mine, src);
+    for (int x = 0;; ++x) {
+      i = (run * steps + x) * 32;
+      cost = cost_of(s, i + lane);
+      incl = scan(cost) + at;
+      const unsigned in = __ballot_sync(0xffffffffu, lo < incl);
+      if (in) {
+        src = __ffs(in) - 1;
+        break;
+      }
+      at = __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
   w.hi = static_cast<int>(min(hi - lo, 0x7fffffffll));
-  w.i = __shfl_sync(0xffffffffu, i0, src);
-  long long at = __shfl_sync(0xffffffffu, incl - mine, src) - lo;  // <= 0
+  w.i = i + src;
+  at = __shfl_sync(0xffffffffu, incl - cost, src) - lo;  // <= 0 from here on
   w.s.row0 = __shfl_sync(0xffffffffu, s.row0, src);
   w.s.n = __shfl_sync(0xffffffffu, s.n, src);
   w.s.len = __shfl_sync(0xffffffffu, s.len, src);
   w.s.slot = __shfl_sync(0xffffffffu, s.slot, src);
-  long long head = 0;
-  while (true) {  // the lane's request, its head, its block
-    if (per > 1) w.s = chunk_seq(a, w.i);
-    head = chunk_head_cost(w.s, bt);
-    if (at + head * a.nkv > 0) break;
-    at += head * a.nkv;
-    ++w.i;
-  }
+  const long long head = chunk_head_cost(w.s, bt);
   for (w.g = 0; at + head <= 0; ++w.g) at += head;
   w.nb = chunk_blocks(w.s.n, bt);
   for (w.k = 0;; ++w.k) {
-    const int cost = chunk_tiles(w.s, w.k, bt) + CHUNK_BLOCK_COST;
-    if (at + cost > 0) break;
-    at += cost;
+    const int c = chunk_tiles(w.s, w.k, bt) + CHUNK_BLOCK_COST;
+    if (at + c > 0) break;
+    at += c;
   }
   w.at = static_cast<int>(at);
   return chunk_fit(a, w, bt);
@@ -269,6 +298,9 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(u)
       : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -413,7 +445,7 @@ constexpr int CHUNK_BLOCKS = 3;
 struct ChunkBars {
   uint64_t q_full[2], q_free[2];               // of a row tile's place
   uint64_t kv_full[CHUNK_K_STAGES + CHUNK_V_STAGES], kv_free[CHUNK_K_STAGES + CHUNK_V_STAGES];  // of K, then of V
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_done[2], o_free[2], merge_full;
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_done[2], o_free[2], ml_full[2];
   uint64_t clear_ask, clear_done;              // rows of a V stage to be zeroed
   uint8_t* clear_at;
   int clear_from;
@@ -431,12 +463,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   using TT = ChunkType<BF16>;
   using T = typename TT::T;
   extern __shared__ __align__(1024) uint8_t chunk_dsmem[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(chunk_dsmem) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = chunk_dsmem;  // (there is no other shared memory: it begins on a 1 KB boundary)
   uint8_t* sm_q = smem;                                    // two row tiles, each [2 halves][128 rows][128 B]
   uint8_t* sm_kv = smem + CHUNK_Q_BYTES;                   // stages of K, then of V: [2 halves][64 positions][128 B]
   uint8_t* sm_out = sm_kv + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES;  // per softmax warp [32 rows][64 B], chunks swizzled
-  float* sm_ml = reinterpret_cast<float*>(sm_out + 8 * CHUNK_OUT_BYTES);  // [2][128]: group 1's m and l
-  ChunkBars& B = *reinterpret_cast<ChunkBars*>(reinterpret_cast<uint8_t*>(sm_ml) + 1024);
+  float* sm_ml = reinterpret_cast<float*>(sm_out + 8 * CHUNK_OUT_BYTES);  // [2 groups][m, l][128]
+  ChunkBars& B = *reinterpret_cast<ChunkBars*>(reinterpret_cast<uint8_t*>(sm_ml) + 2048);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grid = gridDim.x, cta = blockIdx.x;
@@ -459,9 +491,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&B.p_full[i][1], 4);
       mbar_init(&B.pv_done[i][0], 1);
       mbar_init(&B.pv_done[i][1], 1);
-      mbar_init(&B.o_free[i], 4);
+      mbar_init(&B.o_free[i], 8);
+      mbar_init(&B.ml_full[i], 4);
     }
-    mbar_init(&B.merge_full, 4);
     for (int i = 0; i < CHUNK_BLOCKS; ++i) {
       mbar_init(&B.block_full[i], 1);
       mbar_init(&B.block_free[i], 11);
@@ -600,34 +632,33 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         ++n_out;
         tc_fence_after();
       }
+      // two row tiles: each group has its own; one: both groups' results are joined, each group taking 64 dims
       const bool merge = !pair && nt > 1;
-      if (grp == 1 && !pair) {
-        if (had) {  // the first group reads O itself, out of the same lanes
-          sm_ml[row] = m;
-          sm_ml[128 + row] = l;
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B.merge_full);
-        }
-        continue;
-      }
+      if (grp == 1 && !pair && !merge) continue;
+      uint32_t t_a = t_o;
+      float f_a = 1.0f, f_b = 0.0f;
       // a range in which the row saw nothing (m = -inf) is left out of every sum: its O may be anything
-      bool has0 = m != -INFINITY, has1 = false;
-      float f0 = 1.0f, f1 = 0.0f;
+      bool has_a = m != -INFINITY, has_b = false;
       if (merge) {
-        if (!chunk_wait(&B.merge_full, n_merge & 1, abort_flag)) goto softmax_out;
+        sm_ml[grp * 256 + row] = m;
+        sm_ml[grp * 256 + 128 + row] = l;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.ml_full[grp]);
+        if (!chunk_wait(&B.ml_full[grp ^ 1], n_merge & 1, abort_flag)) goto softmax_out;
         ++n_merge;
         tc_fence_after();
-        if (live) {
-          const float m1 = sm_ml[row], l1 = sm_ml[128 + row], top = fmaxf(m, m1);
-          has1 = m1 != -INFINITY;
-          f0 = has0 ? ex2(m - top) : 0.0f;
-          f1 = has1 ? ex2(m1 - top) : 0.0f;
-          l = (has0 ? l * f0 : 0.0f) + (has1 ? l1 * f1 : 0.0f);
-          if (l != l) m = l;
-          else m = top;
-        }
+        const float m_a = sm_ml[row], l_a = sm_ml[128 + row], m_b = sm_ml[256 + row], l_b = sm_ml[384 + row];
+        const float top = fmaxf(m_a, m_b);
+        has_a = m_a != -INFINITY;
+        has_b = m_b != -INFINITY;
+        f_a = has_a ? ex2(m_a - top) : 0.0f;
+        f_b = has_b ? ex2(m_b - top) : 0.0f;
+        l = (has_a ? l_a * f_a : 0.0f) + (has_b ? l_b * f_b : 0.0f);
+        m = l != l ? l : top;
+        t_a = tmem + 256 + lanes;
       }
+      const int c_begin = merge ? 2 * grp : 0, c_end = merge ? c_begin + 2 : 4;  // in 32 dims
       const bool whole = nt == d.tiles;
       const int tok = (pair ? grp * T_tok : 0) + row_tok, pos = d.pos0 + tok;
       const bool seen = pos >= 0;
@@ -637,31 +668,30 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       float bad = 0.0f;
       if (live) {
         const float inv = whole ? 1.0f / l : 1.0f;
-        const float g0 = seen ? f0 * inv : 0.0f, g1 = seen ? f1 * inv : 0.0f;
-        const uint64_t g0x2 = pack2(g0, g0), g1x2 = pack2(g1, g1);
+        const float g_a = seen ? f_a * inv : 0.0f, g_b = seen ? f_b * inv : 0.0f;
+        const uint64_t ga2 = pack2(g_a, g_a), gb2 = pack2(g_b, g_b);
         const unsigned rows_valid = __ballot_sync(0xffffffffu, valid);
-        const bool any1 = __any_sync(0xffffffffu, has1);
         // In nearly every block all rows saw keys in what is joined; where one did not, O may hold anything there.
-        const bool plain = !__any_sync(0xffffffffu, valid && !(seen && has0 && (has1 || !any1)));
+        const bool plain = !__any_sync(0xffffffffu, valid && !(seen && has_a && (has_b || !merge)));
         uint8_t* stage = sm_out + (warp - 4) * CHUNK_OUT_BYTES;
         uint64_t bad2 = 0;
         // dims 32c .. 32c + 31 of this thread's row
         auto fetch = [&](int c, float (&o)[32]) {
-          tmem_ld_x32(t_o + c * 32, o);
-          if (any1) {
+          tmem_ld_x32(t_a + c * 32, o);
+          if (merge) {
             float o1[32];
-            tmem_ld_x32(t_o + 128 + c * 32, o1);
+            tmem_ld_x32(t_a + 128 + c * 32, o1);
             tmem_wait_ld();
             if (!plain) {
 #pragma unroll
               for (int x = 0; x < 32; ++x) {
-                o[x] = has0 ? o[x] : 0.0f;
-                o1[x] = has1 ? o1[x] : 0.0f;
+                o[x] = has_a ? o[x] : 0.0f;
+                o1[x] = has_b ? o1[x] : 0.0f;
               }
             }
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
-              const uint64_t v = fma2(pack2(o1[x], o1[x + 1]), g1x2, mul2(pack2(o[x], o[x + 1]), g0x2));
+              const uint64_t v = fma2(pack2(o1[x], o1[x + 1]), gb2, mul2(pack2(o[x], o[x + 1]), ga2));
               bad2 = fma2(v, 0, bad2);  // NaN once a value is not finite
               unpack2(v, o[x], o[x + 1]);
             }
@@ -669,11 +699,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             tmem_wait_ld();
             if (!plain) {
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = has0 ? o[x] : 0.0f;
+              for (int x = 0; x < 32; ++x) o[x] = has_a ? o[x] : 0.0f;
             }
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
-              const uint64_t v = mul2(pack2(o[x], o[x + 1]), g0x2);
+              const uint64_t v = mul2(pack2(o[x], o[x + 1]), ga2);
               bad2 = fma2(v, 0, bad2);
               unpack2(v, o[x], o[x + 1]);
             }
@@ -695,7 +725,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         if (__popc(rows_valid) <= 4) {  // as in a decode step: a row's stores straight out of its thread are the shorter way
           T* to = static_cast<T*>(a.out) + static_cast<size_t>(out_row) * a.out_ld + qhead * CHUNK_DIM;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
+          for (int c = c_begin; c < c_end; ++c) {
             float o[32];
             fetch(c, o);
             if (!valid) continue;
@@ -714,33 +744,40 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           // output's type, or the partial's in two halves.
           uint4* put = reinterpret_cast<uint4*>(stage + lane * 64);
           const int put_x = lane >> 1 & 3;
-          auto send = [&](auto to) {  // `to`(r, lane's 16-byte chunk) stores row r's chunk lane & 3
+          // lane's rows 8 y + lane / 4, its chunk of each
+          auto send = [&](auto to) {
             __syncwarp();
-#pragma unroll 1
+            uint4 v[4];
+#pragma unroll
             for (int y = 0; y < 4; ++y) {
               const int r = y * 8 + (lane >> 2);
-              to(r, *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) * 16)));
+              v[y] = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) * 16));
             }
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (rows_valid >> (y * 8 + (lane >> 2)) & 1) to(y, v[y]);
             __syncwarp();
           };
           if (whole) {
+            T* to[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int r = y * 8 + (lane >> 2);
+              to[y] = static_cast<T*>(a.out) + static_cast<size_t>(__shfl_sync(0xffffffffu, out_row, r)) * a.out_ld +
+                      __shfl_sync(0xffffffffu, qhead, r) * CHUNK_DIM + (lane & 3) * 8;
+            }
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = c_begin; c < c_end; ++c) {
               float o[32];
               fetch(c, o);
 #pragma unroll
               for (int x = 0; x < 4; ++x) put[x ^ put_x] = pack8(o + 8 * x);
-              send([&](int r, uint4 v) {
-                const int t_row = __shfl_sync(0xffffffffu, out_row, r), t_head = __shfl_sync(0xffffffffu, qhead, r);
-                if (rows_valid >> r & 1)
-                  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<size_t>(t_row) * a.out_ld + t_head * CHUNK_DIM +
-                                            c * 32 + (lane & 3) * 8) = v;
-              });
+              send([&](int y, uint4 v) { *reinterpret_cast<uint4*>(to[y] + c * 32) = v; });
             }
           } else {
-            float* warp_part = my_part - lane * CHUNK_PART_LD;
+            float* to = my_part - lane * CHUNK_PART_LD + (lane >> 2) * CHUNK_PART_LD + (lane & 3) * 4;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = c_begin; c < c_end; ++c) {
               float o[32];
               fetch(c, o);
 #pragma unroll
@@ -750,10 +787,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                   const float* f = o + h * 16 + 4 * x;
                   put[x ^ put_x] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
                 }
-                send([&](int r, uint4 v) {
-                  if (rows_valid >> r & 1)
-                    *reinterpret_cast<uint4*>(warp_part + r * CHUNK_PART_LD + c * 32 + h * 16 + (lane & 3) * 4) = v;
-                });
+                send([&](int y, uint4 v) { *reinterpret_cast<uint4*>(to + y * 8 * CHUNK_PART_LD + c * 32 + h * 16) = v; });
               }
             }
           }
@@ -761,7 +795,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         float b0, b1;
         unpack2(bad2, b0, b1);
         bad = seen ? b0 + b1 : 0.0f;
-        if (valid && !whole) {
+        if (valid && !whole && c_begin == 0) {
           my_part[CHUNK_DIM] = m;
           my_part[CHUNK_DIM + 1] = l;
         }
@@ -769,17 +803,23 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if (had) mbar_arrive(&B.o_free[grp]);
-        if (merge) mbar_arrive(&B.o_free[1]);
+        if (merge) {  // both groups read both
+          mbar_arrive(&B.o_free[0]);
+          mbar_arrive(&B.o_free[1]);
+        } else if (had) {
+          mbar_arrive_n(&B.o_free[grp], 2);
+        }
       }
       // rows that came out not finite, one after the other
       for (unsigned again = __ballot_sync(0xffffffffu, valid && !(bad == 0.0f)); again; again &= again - 1) {
         const int src = __ffs(again) - 1;
         const int r_row = __shfl_sync(0xffffffffu, out_row, src), r_head = __shfl_sync(0xffffffffu, qhead, src);
         const int r_pos = __shfl_sync(0xffffffffu, pos, src), r_prow = __shfl_sync(0xffffffffu, prow, src);
+        const float r_m = __shfl_sync(0xffffffffu, m, src);
         float rm, rl;
         float4 o;
         chunk_row<BF16>(a, d.slot, r_row, r_head, d.t0 * CHUNK_KT, min((d.t0 + nt) * CHUNK_KT, r_pos + 1), rm, rl, o);
+        if (lane >> 3 < c_begin || lane >> 3 >= c_end) continue;  // the other group's dims
         if (whole) {
           const float inv = 1.0f / rl;
           uint2 v;
@@ -787,12 +827,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           v.y = TT::from_f32(o.z * inv, o.w * inv);
           *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(r_row) * a.out_ld + r_head * CHUNK_DIM +
                                     lane * 4) = v;
-        } else {
-          *reinterpret_cast<float4*>(part + r_prow * CHUNK_PART_LD + lane * 4) = o;
-          if (lane == 0) {
-            part[r_prow * CHUNK_PART_LD + CHUNK_DIM] = rm;
-            part[r_prow * CHUNK_PART_LD + CHUNK_DIM + 1] = rl;
-          }
+        } else {  // beside the m and l that are there already
+          const float f = ex2(rm - r_m);
+          *reinterpret_cast<float4*>(part + r_prow * CHUNK_PART_LD + lane * 4) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
         }
       }
       if (!whole && grp == 0 && row == 0) {
