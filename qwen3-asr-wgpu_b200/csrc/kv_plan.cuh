@@ -7,7 +7,9 @@
 // bound by one launch and the few dependent reads below, a large admission by the row maps it
 // writes (8 bytes a row).
 //
-// One cluster does it all.  Every CTA reads the lengths and scans them for itself (a few KB out
+// One cluster does the scans and the pages, and the row maps as well where they are short; long ones (more than
+// PLAN_MAPS_ROWS) are left to kv_row_maps_kernel on all SMs, which expands the finished scan: 8 SMs store
+// 1.1 million rows in 76 us, 148 in a few.  Every CTA of the cluster reads the lengths and scans them for itself (a few KB out
 // of L2, cheaper than handing the sums over); a cluster barrier then stands between the last
 // read and the first write, so that the outputs may be the inputs' own arrays, and the CTAs
 // share the writes.
@@ -20,6 +22,7 @@ namespace qasr {
 
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_MAX_CLUSTER = 8;  // the portable cluster size
+constexpr int PLAN_MAPS_ROWS = 2 * PLAN_MAX_CLUSTER * PLAN_THREADS;
 
 struct PlanArgs {
   const int* seq_slot;
@@ -38,6 +41,7 @@ struct PlanArgs {
   int* row_pos;
   int rows_cap;
   int* status;
+  int maps;  // the row maps are written here
 };
 
 __device__ __forceinline__ void cluster_sync_all() {
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
     else
       a.page_table[line + ((held[lo] + 63) >> 6) + (p - page0[lo])] = a.free_pages[free_count - 1 - p];
   }
-  for (int r = gt; !RELEASE && r < static_cast<int>(rows); r += threads) {
+  for (int r = gt; !RELEASE && a.maps && r < static_cast<int>(rows); r += threads) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -204,6 +208,53 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
     }
     a.row_slot[r] = slot[lo];
     a.row_pos[r] = held[lo] + (r - row0[lo]);
+  }
+}
+
+constexpr int MAPS_THREADS = 256;
+constexpr int MAPS_ROWS = 4;  // consecutive rows of a thread: one 16-byte store to each map
+
+// row_slot / row_pos of the rows that cu_rows gives the requests (none after a refused plan, whose cu_rows are 0).
+__global__ void __launch_bounds__(MAPS_THREADS) kv_row_maps_kernel(const __grid_constant__ PlanArgs a) {
+  extern __shared__ int first_row[];  // [n_seqs + 1]
+  griddep_wait();
+  griddep_launch_dependents();
+  const int n = a.n_seqs;
+  for (int i = threadIdx.x; i <= n; i += MAPS_THREADS) first_row[i] = a.cu_rows[i];
+  __syncthreads();
+  const int rows = min(first_row[n], a.rows_cap);
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.row_slot) | reinterpret_cast<uintptr_t>(a.row_pos)) & 15) == 0;
+  const long long step = static_cast<long long>(gridDim.x) * MAPS_THREADS * MAPS_ROWS;
+  for (long long r0 = (static_cast<long long>(blockIdx.x) * MAPS_THREADS + threadIdx.x) * MAPS_ROWS; r0 < rows; r0 += step) {
+    int lo = 0, hi = n - 1;  // the last request that starts at or before r0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first_row[mid] <= r0) lo = mid; else hi = mid - 1;
+    }
+    int slot[MAPS_ROWS], pos[MAPS_ROWS];
+    int s = a.seq_slot[lo], base = a.kv_len_out[lo] - first_row[lo + 1];  // position of row r: base + r
+#pragma unroll
+    for (int x = 0; x < MAPS_ROWS; ++x) {
+      const int r = static_cast<int>(r0) + x;
+      if (r < rows && r >= first_row[lo + 1]) {
+        do ++lo; while (first_row[lo + 1] <= r);
+        s = a.seq_slot[lo];
+        base = a.kv_len_out[lo] - first_row[lo + 1];
+      }
+      slot[x] = s;
+      pos[x] = base + r;
+    }
+    if (wide && r0 + MAPS_ROWS <= rows) {
+      *reinterpret_cast<int4*>(a.row_slot + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(a.row_pos + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    } else {
+#pragma unroll
+      for (int x = 0; x < MAPS_ROWS; ++x)
+        if (r0 + x < rows) {
+          a.row_slot[r0 + x] = slot[x];
+          a.row_pos[r0 + x] = pos[x];
+        }
+    }
   }
 }
 

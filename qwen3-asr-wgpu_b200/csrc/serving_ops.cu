@@ -119,7 +119,7 @@ qasr_status launch_plan(int device, void* stream, const PlanArgs& a, char* err, 
   cudaError_t e = plan_attrs(device);
   if (e != cudaSuccess) return op_cuda(err, errlen, e, "kernel attributes");
   // one CTA while it can write everything in a few rounds, else a whole cluster
-  const bool small = a.n_seqs <= 256 && (RELEASE || a.rows_cap <= 4 * PLAN_THREADS);
+  const bool small = a.n_seqs <= 256 && (RELEASE || a.rows_cap <= PLAN_THREADS);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(small ? 1 : PLAN_MAX_CLUSTER);
   cfg.blockDim = dim3(PLAN_THREADS);
@@ -135,6 +135,13 @@ qasr_status launch_plan(int device, void* stream, const PlanArgs& a, char* err, 
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   g_launches.fetch_add(1, std::memory_order_relaxed);
   e = cudaLaunchKernelEx(&cfg, kv_plan_kernel<RELEASE>, a);
+  if (e == cudaSuccess && !RELEASE && !a.maps) {
+    const int sms = sm_count(device);
+    const long long ctas = (static_cast<long long>(a.rows_cap) + MAPS_THREADS * MAPS_ROWS - 1) / (MAPS_THREADS * MAPS_ROWS);
+    e = sms <= 0 ? cudaErrorInvalidDevice
+                 : launch_k(kv_row_maps_kernel, dim3(static_cast<unsigned>(std::min<long long>(ctas, sms * 4))), dim3(MAPS_THREADS),
+                            (a.n_seqs + 1) * sizeof(int), static_cast<cudaStream_t>(stream), true, a);
+  }
   return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "kv plan launch");
 }
 
@@ -218,7 +225,7 @@ qasr_status qasr_kernel_kv_plan(int device, void* stream, const int* seq_slot, c
       !row_slot || !row_pos || !status || rows_cap < 0 || bad_plan_sizes(n_seqs, max_slots, max_pages, pool_pages))
     return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad kv plan arguments");
   PlanArgs a{seq_slot, kv_len, new_len, n_seqs, max_slots, page_table, max_pages, const_cast<int*>(free_pages),
-             pool_pages, free_count, kv_len_out, free_count_out, cu_rows, row_slot, row_pos, rows_cap, status};
+             pool_pages, free_count, kv_len_out, free_count_out, cu_rows, row_slot, row_pos, rows_cap, status, rows_cap <= PLAN_MAPS_ROWS};
   return launch_plan<false>(device, stream, a, err, errlen);
 }
 
@@ -230,7 +237,7 @@ qasr_status qasr_kernel_kv_release(int device, void* stream, const int* seq_slot
       bad_plan_sizes(n_seqs, max_slots, max_pages, pool_pages))
     return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad kv release arguments");
   PlanArgs a{seq_slot, kv_len, nullptr, n_seqs, max_slots, const_cast<int*>(page_table), max_pages, free_pages,
-             pool_pages, free_count, kv_len_out, free_count_out, nullptr, nullptr, nullptr, 0, status};
+             pool_pages, free_count, kv_len_out, free_count_out, nullptr, nullptr, nullptr, 0, status, 0};
   return launch_plan<true>(device, stream, a, err, errlen);
 }
 

@@ -95,6 +95,37 @@ def test_kv_plan_matches_a_plain_allocator(qasr, cuda_device, n, slots, hi, alia
         held = got["out"]
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+def test_kv_plan_long_row_maps(qasr, cuda_device, shift):
+    """More rows than the planning cluster writes itself, runs of empty requests among them, maps on and off 16-byte
+    boundaries, and more room than rows."""
+    import torch
+    rng = random.Random(shift)
+    n, max_pages = 400, 40
+    new = [rng.choice([0, 0, 1, 3, 64, 2000, rng.randint(0, 300)]) for _ in range(n)]
+    new[:5], new[-6:] = [0] * 5, [0] * 6
+    held = [rng.randint(0, 500) for _ in range(n)]
+    assert sum(new) > 40000
+    p = Pages(torch, n, max_pages, n * max_pages, seed=2)
+    slot = rng.sample(range(n), n)
+    first = p.plan(qasr, slot, [0] * n, held)
+    _check_plan(p, first, slot, [0] * n, held)
+    cu, rs, rp = p.expect(slot, held, new)
+    s, h, a = _ints(slot, torch), _ints(held, torch), _ints(new, torch)
+    maps = [torch.full((len(rs) + 100,), -9, dtype=torch.int32, device="cuda") for _ in range(2)]
+    d_cu, st = _ints([0] * (n + 1), torch), _ints([-9, -9], torch)
+    qasr.kernel_kv_plan(0, _stream(torch), s.data_ptr(), h.data_ptr(), a.data_ptr(), n, n, p.d_table.data_ptr(), max_pages,
+                        p.d_free.data_ptr(), p.pool_pages, p.d_count.data_ptr(), h.data_ptr(), p.d_count.data_ptr(),
+                        d_cu.data_ptr(), maps[0].data_ptr() + 4 * shift, maps[1].data_ptr() + 4 * shift, len(rs) + 90,
+                        st.data_ptr())
+    torch.cuda.synchronize()
+    assert st.tolist() == [0, 0] and d_cu.tolist() == cu and p.d_count.item() == len(p.free)
+    for got, want in zip(maps, (rs, rp)):
+        got = got.tolist()
+        assert got[shift:shift + len(want)] == want and set(got[shift + len(want):] + got[:shift]) == {-9}
+    assert p.d_table.tolist() == p.table and h.tolist() == [x + y for x, y in zip(held, new)]
+
+
 def test_kv_plan_without_new_lengths_adds_one_each(qasr, cuda_device):
     import torch
     p = Pages(torch, 9, 4, 30)
