@@ -77,7 +77,7 @@ constexpr int CHUNK_Q_TILE = 128 * CHUNK_DIM * 2, CHUNK_Q_HALF = CHUNK_Q_TILE / 
 constexpr int CHUNK_Q_BYTES = 2 * CHUNK_Q_TILE;
 constexpr int CHUNK_OUT_BYTES = 32 * 64;           // per softmax warp: a quarter of its rows' output
 constexpr int CHUNK_SMEM = CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 3072;
-constexpr int CHUNK_BLOCK_COST = 2;               // a block's Q copy, first and last steps, in key tiles
+constexpr int CHUNK_BLOCK_COST = 4;               // a block's Q copy, first and last steps, in key tiles
 constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
 constexpr uint32_t CHUNK_WAIT_STEPS = (10 * QASR_WAIT_NS) >> 20;  // rows computed again by chunk_row keep the others waiting

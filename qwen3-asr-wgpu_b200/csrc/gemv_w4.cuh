@@ -175,7 +175,7 @@ constexpr int W4_MAX_CLUSTER = 4;
 template <bool ZERO, int GS, int NT>
 struct W4Plan {
   static constexpr int unit_bytes = 2048 + GS * 64 + (ZERO ? GS * 32 : 0);
-  static constexpr int per_sm = NT == 1 ? 3 : NT == 8 ? 1 : 2;  // resident CTAs, by their registers
+  static constexpr int per_sm = NT == 1 ? 3 : NT == 2 ? 2 : 1;  // resident CTAs, by their registers
   static constexpr int bufs = NT <= 2 ? 2 : 1;
   static constexpr int sums_bytes = bufs * W4_WARPS * 8 * NT * 33 * 4;
   static constexpr int bars_bytes = 512;
@@ -247,6 +247,24 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
       xr[n] = static_cast<const T*>(a.x) + static_cast<long long>(min(n * 8 + (lane >> 2), a.rows - 1)) * a.ldx + t * 8;
     float acc[2][NT][4];
     // a unit's products; the last one of a k that is no multiple of 128 lacks some of its 32-column quarters
+    // At 32 rows and below a unit's share of x is asked for before its weights are waited for.
+    constexpr bool PRE = NT <= 4;
+    uint4 px[PRE ? 4 : 1][NT];
+    auto fetch_x = [&](int u) {
+      const int left = a.k - u * 128;
+      if (left >= 128) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int m = 0; m < NT; ++m) px[q][m] = __ldg(reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32));
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int m = 0; m < NT; ++m)
+            px[q][m] = q * 32 < left ? __ldg(reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32)) : make_uint4(0, 0, 0, 0);
+      }
+    };
     auto product = [&](auto whole, int u, const uint8_t* unit) {
       constexpr bool FULL = decltype(whole)::value;
       const uint4* codes = reinterpret_cast<const uint4*>(unit) + lane;
@@ -261,8 +279,10 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
         constexpr int per = 4 / GS;  // quarters under one scale
         uint4 xv[NT];
 #pragma unroll
-        for (int m = 0; m < NT; ++m)
-          xv[m] = FULL || q * 32 < left ? __ldg(reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32)) : make_uint4(0, 0, 0, 0);
+        for (int m = 0; m < NT; ++m) {
+          if (PRE) xv[m] = px[q][m];
+          else xv[m] = FULL || q * 32 < left ? __ldg(reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32)) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (q % 2 == 0) w[i] = codes[i * 64 + q / 2 * 32];
@@ -306,12 +326,13 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
         for (int m = 0; m < NT; ++m) acc[i][m][0] = acc[i][m][1] = acc[i][m][2] = acc[i][m][3] = 0.0f;
       if (g * wt_n + wt < L.tiles) {
         for (int u = u0; u < u1 && !lost; u += wk_n) {
+          if constexpr (PRE) fetch_x(u);
           if (!__all_sync(0xffffffffu, mbar_try_wait(&full[slot], parity)) &&
               !mbar_wait_warp(&full[slot], parity, abort_flag, nullptr, 0)) {
             lost = true;
             break;
           }
-          if (u * 128 + 128 <= a.k) product(std::true_type{}, u, ring + slot * P::unit_bytes);
+          if (PRE || u * 128 + 128 <= a.k) product(std::true_type{}, u, ring + slot * P::unit_bytes);
           else product(std::false_type{}, u, ring + slot * P::unit_bytes);
           __syncwarp();
           if (lane == 0) copy_next(static_cast<int>(slot));  // into the slot that was read just now

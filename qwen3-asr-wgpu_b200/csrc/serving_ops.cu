@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -75,10 +76,13 @@ cudaError_t plan_attrs(int device) noexcept {
 }
 
 int sm_count(int device) noexcept {
-  int n = 0;
-  if (device < 0 || device >= kMaxDevices ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    return -1;
+  static std::atomic<int> known[kMaxDevices];
+  if (device < 0 || device >= kMaxDevices) return -1;
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return -1;
+    known[device].store(n, std::memory_order_relaxed);
+  }
   return n;
 }
 
