@@ -166,9 +166,13 @@ cudaError_t launch_w4_kernel(W4Args a, int device, int sms, cudaStream_t st) {
   const auto kernel = gemv_w4_kernel<BF16, ZERO, GS, NT>;
   static std::once_flag once[kMaxDevices];
   static cudaError_t ready[kMaxDevices] = {};
-  std::call_once(once[device], [kernel, device] {
-    ready[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::smem);
-  });
+  try {
+    std::call_once(once[device], [kernel, device] {
+      ready[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::smem);
+    });
+  } catch (...) {
+    return cudaErrorUnknown;
+  }
   if (ready[device] != cudaSuccess) return ready[device];
   const W4Layout L = w4_layout(a.n_out, a.k, 128 / GS, ZERO);
   a.wk_log2 = 3;

@@ -524,6 +524,44 @@ def test_chunk_attention_captured_and_replayed_with_other_lengths(qasr, cuda_dev
     c.check(c.out)
 
 
+@pytest.mark.parametrize("n", [33, 1000, 1025, 2500])
+def test_chunk_attention_many_requests(qasr, cuda_device, n):
+    """As many requests as the schedule reads in one, two and several steps, empty ones and chunks among them."""
+    import torch
+    rng = random.Random(n)
+    lens = [(rng.randint(0, 40), rng.choice([0, 1, 1, 1, 2, 5])) for _ in range(n)]
+    lens[n // 2] = (300, 200)
+    c = Chunks(torch, lens, nq=8, nkv=4, seed=n)
+    ws = c.workspace(qasr)
+    out = c.run(qasr, ws=ws)
+    qasr.kernel_attention_chunk_check(0, _stream(torch), ws[0].data_ptr())
+    c.check(out)
+
+
+def test_chunk_attention_very_many_tiles(qasr, cuda_device):
+    """More than 2^22 key tiles in one call (requests that share their pages), where cuts are placed in 64 bits."""
+    import torch
+    n, ctx = 4200, 8191
+    c = Chunks(torch, [(ctx, 1)], seed=18)
+    c.n = c.slots = n
+    c.table = c.table[c.slot[0].long()].repeat(n, 1)
+    c.slot = torch.arange(n, dtype=torch.int32, device="cuda")
+    c.cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    c.kv_len = torch.full((n,), ctx + 1, dtype=torch.int32, device="cuda")
+    c.cap = n
+    c.q = c.q[:1].repeat(n, 1)
+    out = c.run(qasr, out=torch.full((n, 2048), 77.0, dtype=torch.float16, device="cuda"))
+    torch.cuda.synchronize()
+    got = torch.full((2, 2048), 77.0, dtype=torch.float16, device="cuda")
+    for r in (0, 1, n // 2, n - 1):
+        got[0] = out[r]
+        c.check(got)
+    # every row against the first: two errors of at most u|o| and u A each (with the terms of `check` that are small here),
+    # A = sum p|v| / sum p being an average of |v| over 8192 keys, below 1
+    first = out[:1].float()
+    assert ((out.float() - first).abs() <= 2 * 2.0 ** -11 * 1.1 * (first.abs() + 1)).all()
+
+
 def test_chunk_attention_small_workspace_is_refused(qasr, cuda_device):
     import torch
     c = Chunks(torch, [(0, 4)])
