@@ -859,12 +859,17 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mbar_arrive(&B.block_free[n % CHUNK_BLOCKS]);
         const int place = pair ? 0 : n & 1;  // of Q; a pair takes both
         bool ok = true;
-        for (int x = place; x < (pair ? 2 : place + 1); ++x) ok = ok && wait_one(&B.q_full[x], n_q[x]++ & 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (pair || x == place) ok = ok && wait_one(&B.q_full[x], n_q[x]++ & 1);
         for (int j = 0; ok && j < nt; ++j) {
           if (!(ok = wait_one(&B.kv_full[st], parity))) break;
           const uint64_t dk = desc_k + st * (CHUNK_STAGE_BYTES >> 4);
           // a pair's groups share the key tiles; those of a one-tile block take them in turn
-          for (int g = pair ? static_cast<int>(j >= nt0) : j & 1; g < (pair ? 2 : (j & 1) + 1); ++g) {
+          const int who = pair ? (j < nt0 ? 3 : 2) : 1 << (j & 1);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!(who >> g & 1)) continue;
             const uint32_t c = n_s[g]++, buf = c & 1;
             // the buffer's last P has been read
             if (c >= 2 && !(ok = wait_one(&B.pv_done[g][buf], ((c >> 1) - 1) & 1))) break;
@@ -910,7 +915,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             if (!(ok = wait_one(&B.clear_done, n_clear++ & 1))) break;
           }
           const uint64_t dv = desc_v + st * (CHUNK_STAGE_BYTES >> 4);
-          for (int g = pair ? static_cast<int>(j >= nt0) : j & 1; g < (pair ? 2 : (j & 1) + 1); ++g) {
+          const int who = pair ? (j < nt0 ? 3 : 2) : 1 << (j & 1);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!(who >> g & 1)) continue;
             const bool first = pair ? j == 0 : j < 2, last = pair ? j == (g ? nt : nt0) - 1 : j + 2 >= nt;
             // the block before has been read out
             if (first && n_out[g]++ && !(ok = wait_one(&B.o_free[g], n_out[g] & 1))) break;
