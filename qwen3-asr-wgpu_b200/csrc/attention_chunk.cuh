@@ -14,9 +14,9 @@
 // A page's swizzle (chunk c of position p at c ^ (p % 8)) is, for each 64-dim half of its rows, the
 // tensor core's own 128-byte swizzle, so pages are copied by TMA as they are and used as operands.
 // Tensor memory holds two S tiles and O of each row tile: while a tile's softmax runs, the next tile's
-// product is under way, so the softmax never waits for it.  (Two S tiles of 128 keys would not fit beside O; of 64 keys
-// Q K^T runs at 3/4 of the tensor cores' rate, its operands coming from shared memory, which costs less than the
-// wait: one S tile of 128 keys ran at 4050 cycles per 128 keys and two row tiles, half of them waiting.)
+// product is under way.  (Two S tiles of 128 keys would not fit beside O.  Of 64 keys Q K^T runs at 3/4 of the tensor
+// cores' rate, its operands coming from shared memory, and still costs less than the wait for the only S tile of 128: 8192
+// rows took 293 us that way.)
 // P is rounded to the cache's type for the second product, as the tensor core wants it; the sum of P
 // is taken before that rounding.  m is raised, and O rescaled, only when a row's maximum has grown by more than
 // 2^8 (P then stays below 2^8, far inside f16), so the rescaling, a round trip over O, is rare.
@@ -33,6 +33,12 @@
 // laid end to end, are cut into one equal range per CTA.  A block that a cut goes through leaves f32
 // partials (o, m, l) in the workspace and attention_chunk_combine_kernel joins them, in key order.
 // Nothing about the lengths is known on the host: every CTA sums the costs itself.
+//
+// Measured (B200, us in a graph): 512 slots of 256-4096 positions 690-735 (6.1-6.5 TB/s, 94-99% of the measured copy rate),
+// 32 slots of 100-1500 31, one token over 224 positions 10.6 (latency: launch 2, first block found 3, pages 1, three
+// dependent products and softmaxes 3, join 2), 64 requests of 13 rows 64-74, 8192 rows from nothing 261 (1050
+// TFLOP/s, 64% of measured bf16): the chain P -> P V -> Q K^T -> S of each group takes about 1950 cycles for 64 keys where the
+// tensor cores need 1280 for both groups' products and the exponentials 1024.
 //
 // Masked keys: S is replaced, never added to, so whatever stands there cannot matter; their P is 0, and
 // V rows behind the block's last position are zeroed in shared memory, so that 0 * NaN cannot arise.  What remains
@@ -77,7 +83,7 @@ constexpr int CHUNK_Q_TILE = 128 * CHUNK_DIM * 2, CHUNK_Q_HALF = CHUNK_Q_TILE / 
 constexpr int CHUNK_Q_BYTES = 2 * CHUNK_Q_TILE;
 constexpr int CHUNK_OUT_BYTES = 32 * 64;           // per softmax warp: a quarter of its rows' output
 constexpr int CHUNK_SMEM = CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 3072;
-constexpr int CHUNK_BLOCK_COST = 4;               // a block's Q copy, first and last steps, in key tiles
+constexpr int CHUNK_BLOCK_COST = 4;               // a block's Q copy, first and last steps, in key tiles (2: 32 slots 33.7 us, 4: 30.9, 6: 31.6)
 constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
 constexpr uint32_t CHUNK_WAIT_STEPS = (10 * QASR_WAIT_NS) >> 20;  // rows computed again by chunk_row keep the others waiting
@@ -722,7 +728,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           return v;
         };
         float* my_part = part + prow * CHUNK_PART_LD;
-        if (__popc(rows_valid) <= 4) {  // as in a decode step: a row's stores straight out of its thread are the shorter way
+        if (__popc(rows_valid) <= 4) {  // as in a decode step: straight out of the rows' threads (32 slots: 31.1 us, through shared memory 32.2)
           T* to = static_cast<T*>(a.out) + static_cast<size_t>(out_row) * a.out_ld + qhead * CHUNK_DIM;
 #pragma unroll 1
           for (int c = c_begin; c < c_end; ++c) {

@@ -122,8 +122,9 @@ qasr_status launch_plan(int device, void* stream, const PlanArgs& a, char* err, 
   if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
   cudaError_t e = plan_attrs(device);
   if (e != cudaSuccess) return op_cuda(err, errlen, e, "kernel attributes");
-  // one CTA while it can write everything in a few rounds, else a whole cluster
-  const bool small = a.n_seqs <= 256 && (RELEASE || a.rows_cap <= PLAN_THREADS);
+  // One CTA while it writes everything in a round or two, else a whole cluster (us in a graph, one CTA / eight: 8000
+  // rows 5.9 / 3.7; 200 requests released, 2600 pages, 5.1 / 3.6; a decode step of 32 needs no more than one: 3.8).
+  const bool small = RELEASE ? a.n_seqs <= 64 : a.n_seqs <= 256 && a.rows_cap <= PLAN_THREADS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(small ? 1 : PLAN_MAX_CLUSTER);
   cfg.blockDim = dim3(PLAN_THREADS);
@@ -177,9 +178,11 @@ cudaError_t launch_w4_kernel(W4Args a, int device, int sms, cudaStream_t st) {
   const W4Layout L = w4_layout(a.n_out, a.k, 128 / GS, ZERO);
   a.wk_log2 = 3;
   while ((1 << a.wk_log2) > L.units) --a.wk_log2;
-  // Few row tiles: two or four CTAs share each, as long as they fit the SMs and every warp still has a unit.
+  // Few row tiles and a long k: two or four CTAs share each tile, as long as they fit the SMs and every warp keeps a few
+  // units (us, alone / shared: 2048 x 6144 at one row 5.3 / 4.4, at 32 rows 10.6 / 9.0; 2048 x 2048, where a warp would
+  // be left with one unit, 2.8 / 3.15).
   a.cluster = 1;
-  while (a.cluster < W4_MAX_CLUSTER && L.tiles * a.cluster * 2 <= sms && L.units >= 16 * a.cluster) a.cluster *= 2;
+  while (a.cluster < W4_MAX_CLUSTER && L.tiles * a.cluster * 2 <= sms && L.units >= 32 * a.cluster) a.cluster *= 2;
   const int per_cta = W4_WARPS >> a.wk_log2;
   const int groups = (L.tiles + per_cta - 1) / per_cta;
   cudaLaunchConfig_t cfg = {};
