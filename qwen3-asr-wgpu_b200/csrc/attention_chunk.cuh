@@ -993,7 +993,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           id1 = id2;
           id2 = next;
           if (j < nt) {
-            if (j + 1 < have) next = j + 1 < 16 ? d.pages[j + 1] : __ldg(table + j + 1);
+            if (j + 1 < have) next = j + 1 < 16 ? d.pages[j + 1] : table[j + 1];
             ok = load_page(st_k, lap_k, id2, row_k, j < have);
             if (++st_k == CHUNK_K_STAGES) {
               st_k = 0;

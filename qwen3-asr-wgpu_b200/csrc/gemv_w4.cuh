@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
       xr[n] = static_cast<const T*>(a.x) + static_cast<long long>(min(n * 8 + (lane >> 2), a.rows - 1)) * a.ldx + t * 8;
     float acc[2][NT][4];
     // a unit's products; the last one of a k that is no multiple of 128 lacks some of its 32-column quarters
-    // At 32 rows and below a unit's share of x is asked for before its weights are waited for.
+    // At 32 rows and below a unit's share of x is asked for before its weights are waited for.  (Plain loads: the kernel may
+    // have started while x was still being written, so it is not read-only for its whole life.)
     constexpr bool PRE = NT <= 4;
     uint4 px[PRE ? 4 : 1][NT];
     auto fetch_x = [&](int u) {
@@ -258,13 +259,13 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int m = 0; m < NT; ++m) px[q][m] = __ldg(reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32));
+          for (int m = 0; m < NT; ++m) px[q][m] = *reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32);
       } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int m = 0; m < NT; ++m)
-            px[q][m] = q * 32 < left ? __ldg(reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32)) : make_uint4(0, 0, 0, 0);
+            px[q][m] = q * 32 < left ? *reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32) : make_uint4(0, 0, 0, 0);
       }
     };
     auto product = [&](auto whole, int u, const uint8_t* unit) {
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
 #pragma unroll
         for (int m = 0; m < NT; ++m) {
           if (PRE) xv[m] = px[q][m];
-          else xv[m] = FULL || q * 32 < left ? __ldg(reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32)) : make_uint4(0, 0, 0, 0);
+          else xv[m] = FULL || q * 32 < left ? *reinterpret_cast<const uint4*>(xr[m] + u * 128 + q * 32) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
