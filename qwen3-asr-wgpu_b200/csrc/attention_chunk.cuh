@@ -36,9 +36,9 @@
 //
 // Measured (B200, us in a graph): 512 slots of 256-4096 positions 690-735 (6.1-6.5 TB/s, 94-99% of the measured copy rate),
 // 32 slots of 100-1500 31, one token over 224 positions 10.6 (latency: launch 2, first block found 3, pages 1, three
-// dependent products and softmaxes 3, join 2), 64 requests of 13 rows 64-74, 8192 rows from nothing 261 (1050
-// TFLOP/s, 64% of measured bf16): the chain P -> P V -> Q K^T -> S of each group takes about 1950 cycles for 64 keys where the
-// tensor cores need 1280 for both groups' products and the exponentials 1024.
+// dependent products and softmaxes 3, join 2), 64 requests of 13 rows 62-74, 8192 rows from nothing 247 (1110
+// TFLOP/s, 68% of measured bf16): the chain P -> P V -> Q K^T -> S of each group takes about 1850 cycles for 64 keys where the
+// tensor cores need 1280 for both groups' products and the exponential unit 768.
 //
 // Masked keys: S is replaced, never added to, so whatever stands there cannot matter; their P is 0, and
 // V rows behind the block's last position are zeroed in shared memory, so that 0 * NaN cannot arise.  What remains
@@ -341,6 +341,29 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// 2^x for two x <= 2^8 on the FMA pipe: x = n + f with n the nearest integer, 2^f by the polynomial of degree 4 with the
+// smallest largest relative error on [-1/2, 1/2] and value 1 at 0 (2.9e-6 in f32, found by weighted least squares; f16 rounds P
+// to 4.9e-4), n added to the exponent.  At -127 and below, a masked score's -inf among them, the result is exactly 0.  What is
+// not a number becomes 2^128 or more once rounded, so the row comes out not finite and is computed again (chunk_row).
+__device__ __forceinline__ void ex2_poly2(uint64_t x2, float& a, float& b) {
+  float xa, xb;
+  unpack2(x2, xa, xb);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(xa) : "f"(-127.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(xb) : "f"(-127.0f));
+  x2 = pack2(xa, xb);
+  const uint64_t magic = pack2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are the integer
+  const uint64_t t = add2(x2, magic);
+  const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x2);
+  uint64_t p = fma2(pack2(0.009582853f, 0.009582853f), f, pack2(0.055906426f, 0.055906426f));
+  p = fma2(p, f, pack2(0.24024099f, 0.24024099f));
+  p = fma2(p, f, pack2(0.69312418f, 0.69312418f));
+  p = fma2(p, f, pack2(1.0f, 1.0f));
+  float ta, tb, pa, pb;
+  unpack2(t, ta, tb);
+  unpack2(p, pa, pb);
+  a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
+}
 // Shared-memory descriptor of V as the second operand, MN-major with 128-byte swizzle: 64-dim halves
 // CHUNK_HALF_BYTES apart (LBO), groups of 8 positions 1024 bytes apart (SBO).
 __device__ __forceinline__ uint64_t smem_desc_v(uint32_t smem_addr) {
@@ -614,9 +637,17 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           uint32_t p[32];
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
-            float e0, e1;
-            unpack2(fma2(pack2(s[2 * c], s[2 * c + 1]), scale2, base2), e0, e1);
-            const float p0 = ex2(e0), p1 = ex2(e1);
+            // every fourth pair on the FMA pipe, so that the exponential unit is not what a tile waits for (8192 rows: none
+            // 261 us, a fourth 247, a third 250)
+            const uint64_t e = fma2(pack2(s[2 * c], s[2 * c + 1]), scale2, base2);
+            float p0, p1;
+            if (c % 4 == 3) {
+              ex2_poly2(e, p0, p1);
+            } else {
+              unpack2(e, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+            }
             sum[c & 1] = add2(sum[c & 1], pack2(p0, p1));
             p[c] = TT::from_f32(p0, p1);
           }

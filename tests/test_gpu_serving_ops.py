@@ -440,6 +440,40 @@ def test_chunk_attention_later_positions_do_not_reach_earlier_rows(qasr, cuda_de
         assert out[150:200, :c.nq * DIM].isnan().all() and out[239, :c.nq * DIM].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("at", [64 + x for x in range(8)] + [127, 130])
+def test_chunk_attention_a_key_that_is_not_a_number_shows_in_every_row_that_sees_it(qasr, cuda_device, at, dtype):
+    """Whatever column of a tile it stands in: a chunk of two row tiles, a cut decode row and a short chunk."""
+    import torch
+    c = Chunks(torch, [(0, 150), (1000, 1), (120, 20)], seed=19, dtype=dtype)
+    kv = [x.clone() for x in c.kv]
+    for x in c.kv:
+        x[0, :, at] = float("nan")
+    c.store()
+    out = c.run(qasr)
+    torch.cuda.synchronize()
+    seen = set(range(at, 150)) | {150} | {151 + j for j in range(20) if 120 + j >= at}
+    for r in seen:
+        assert out[r, :2048].isnan().all(), r
+    c.kv = kv
+    c.check(out, skip=seen)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_chunk_attention_huge_values_at_masked_positions(qasr, cuda_device, dtype):
+    """The largest finite values at later positions: a masked probability is exactly 0."""
+    import torch
+    c = Chunks(torch, [(64, 128), (10, 60)], seed=20, dtype=dtype)
+    kv = [x.clone() for x in c.kv]
+    for x in c.kv:
+        x[1, :, -60:] = torch.finfo(c.t).max
+    c.store()
+    out = c.run(qasr)
+    torch.cuda.synchronize()
+    c.kv = kv
+    c.check(out, skip=set(range(68, 128)) | set(range(128, 188)))
+
+
 def test_chunk_attention_rows_that_see_nothing(qasr, cuda_device):
     """More rows than positions: the rows before position 0 are zeros; a request without any position too."""
     import torch
