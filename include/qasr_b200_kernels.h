@@ -222,7 +222,8 @@ qasr_status qasr_kernel_pack_w4(int device, void* stream, const uint8_t* codes, 
  * out[r, m] = type(f32(out[r, m]) + sum_c W[m, c] x[r, c])         (accumulate != 0)
  * for 1 <= rows <= QASR_W4_MAX_ROWS; x [rows, ldx], out [rows, ldo] of `type`, ldx >= k a multiple
  * of 8, ldo >= n_out, x on a 16-byte boundary; out may overlap neither x nor packed.  Codes and zero
- * points enter the product exactly, each group's sum and the sum over groups are f32. */
+ * points enter the product exactly, each group's sum and the sum over groups are f32.
+ * Only enqueues: a bounded device-side wait for its own copies that gives up is not reported. */
 qasr_status qasr_kernel_gemv_w4(int device, void* stream, int type, const void* packed, int has_zero,
                                 int n_out, int k, int group, const void* x, int ldx, int rows, void* out,
                                 int ldo, int accumulate, char* err, int errlen);
