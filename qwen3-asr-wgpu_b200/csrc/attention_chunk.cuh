@@ -82,7 +82,7 @@ constexpr int CHUNK_HALF_BYTES = CHUNK_KT * 128;  // the rows' first or second 6
 constexpr int CHUNK_Q_TILE = 128 * CHUNK_DIM * 2, CHUNK_Q_HALF = CHUNK_Q_TILE / 2;
 constexpr int CHUNK_Q_BYTES = 2 * CHUNK_Q_TILE;
 constexpr int CHUNK_OUT_BYTES = 32 * 64;           // per softmax warp: a quarter of its rows' output
-constexpr int CHUNK_SMEM = CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 3072;
+constexpr int CHUNK_SMEM = CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 3 * 1024;  // (m and l, ChunkBars)
 constexpr int CHUNK_BLOCK_COST = 4;               // a block's Q copy, first and last steps, in key tiles (2: 32 slots 33.7 us, 4: 30.9, 6: 31.6)
 constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
