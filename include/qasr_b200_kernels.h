@@ -106,7 +106,8 @@ qasr_status qasr_kernel_attention_noalloc(int device, void* stream, const uint16
 
 /* Append K and V rows ([rows, nkv*128] f16 each) at (row_slot[r], row_pos[r]) of
  * layer `layer`, in the swizzled row layout qasr_kernel_attention reads — the cache
- * writes of qkv_extract(_slots) (src/shaders.rs:1376-1635). */
+ * writes of qkv_extract(_slots) (src/shaders.rs:1376-1635).  All `rows` are written and their maps and the
+ * table taken as given; a step planned on the device has qasr_kernel_kv_append_planned. */
 qasr_status qasr_kernel_kv_append(int device, void* stream, const uint16_t* k, const uint16_t* v,
                                   uint16_t* kv_pool, const int* page_table, int max_pages,
                                   int layers, int nkv, int layer, const int* row_slot,
@@ -115,7 +116,7 @@ qasr_status qasr_kernel_kv_append(int device, void* stream, const uint16_t* k, c
 /* ------------------------------------------------------------------ serving over the paged cache
  * A serving step on the device, with no read-back of lengths to the host: qasr_kernel_kv_plan
  * gives each request the pages and row maps of its new positions, the projections may read 4-bit
- * weights (qasr_kernel_gemv_w4), qasr_kernel_kv_append writes the new rows, and
+ * weights (qasr_kernel_gemv_w4), qasr_kernel_kv_append_planned writes the new rows, and
  * qasr_kernel_attention_chunk attends them.  No counterpart in the reference, whose decoder
  * keeps one contiguous cache per slot (fork_capped, src/decoder.rs:2453).
  * These calls allocate nothing and keep nothing between calls, so they may be captured into a
@@ -150,7 +151,10 @@ enum {
  *     positions; -1: the free stack is too short; -2: more rows than rows_cap.
  * (Invalid arguments come before capacity, the requests before -1, -1 before -2.)
  * Then every cu_rows entry is 0 (the step has no rows), kv_len_out = kv_len, free_count_out =
- * free_count and nothing else is written.  The page ids on the stack are taken as given.
+ * free_count and nothing else is written: the row maps then still hold an earlier step's rows, as their
+ * entries behind the last row always do, so what writes through them has to stop at
+ * cu_rows[n_seqs] rows (qasr_kernel_kv_append_planned does; qasr_kernel_kv_append writes the `rows`
+ * that it is told).  The page ids on the stack are taken as given.
  * n_seqs <= QASR_KV_PLAN_MAX_SEQS, max_slots <= QASR_KV_PLAN_MAX_SLOTS, max_pages < 2^25. */
 qasr_status qasr_kernel_kv_plan(int device, void* stream, const int* seq_slot, const int* kv_len,
                                 const int* new_len, int n_seqs, int max_slots, int* page_table,
@@ -169,6 +173,18 @@ qasr_status qasr_kernel_kv_release(int device, void* stream, const int* seq_slot
                                    int* free_pages, int pool_pages, const int* free_count,
                                    int* kv_len_out, int* free_count_out, int* status, char* err,
                                    int errlen);
+
+/* Append the new K and V rows of a planned step ([rows_cap, nkv * 128] each, f16 or bf16) to layer `layer` of the
+ * cache: row r goes to (row_slot[r], row_pos[r]) as in qasr_kernel_kv_append, for 0 <= r < min(*row_count,
+ * rows_cap).  row_count is a device int, cu_rows + n_seqs of the plan: rows that the plan did not give out
+ * (all of them after a refused one) are neither read nor written, whatever the maps hold there.  A row whose
+ * slot, position or page lies outside [0, max_slots), [0, max_pages * 64), [0, pool_pages) is left out.
+ * k, v and kv_pool on 16-byte boundaries; kv_pool and page_table as in qasr_kernel_attention_chunk. */
+qasr_status qasr_kernel_kv_append_planned(int device, void* stream, const uint16_t* k, const uint16_t* v,
+                                          uint16_t* kv_pool, int pool_pages, const int* page_table,
+                                          int max_slots, int max_pages, int layers, int nkv, int layer,
+                                          const int* row_slot, const int* row_pos, int rows_cap,
+                                          const int* row_count, char* err, int errlen);
 
 /* GQA attention of chunks of new tokens over the paged cache.  Request i has the query rows
  * cu_rows[i] .. cu_rows[i+1]-1 and kv_len[i] cached positions, its new ones among them (what

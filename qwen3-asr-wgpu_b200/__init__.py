@@ -61,7 +61,7 @@ EXPORTED_SYMBOLS = (
     "qasr_kernel_pack_weights", "qasr_kernel_gemm", "qasr_kernel_gemm_traced", "qasr_kernel_attention",
     "qasr_kernel_attention_noalloc", "qasr_kernel_attention_traced", "qasr_kernel_kv_append",
     "qasr_kernel_launch_count",
-    "qasr_kernel_kv_plan", "qasr_kernel_kv_release", "qasr_kernel_attention_chunk_workspace",
+    "qasr_kernel_kv_plan", "qasr_kernel_kv_release", "qasr_kernel_kv_append_planned", "qasr_kernel_attention_chunk_workspace",
     "qasr_kernel_attention_chunk", "qasr_kernel_attention_chunk_check", "qasr_kernel_w4_packed_bytes", "qasr_kernel_pack_w4", "qasr_kernel_gemv_w4",
     "qasr_synth_key", "qasr_synth_normal_f16", "qasr_synth_uniform_ids",
     "qasr_synth_quantize_rows", "qasr_f32_to_f16", "qasr_f16_to_f32", "qasr_f32_to_f16_array",
@@ -274,6 +274,7 @@ def _load() -> ctypes.CDLL:
     lib.qasr_kernel_launch_count.restype = ctypes.c_uint64
     lib.qasr_kernel_kv_plan.argtypes = [I, P, P, P, P, I, I, P, I, P, I, P, P, P, P, P, P, I, P, ctypes.c_char_p, I]
     lib.qasr_kernel_kv_release.argtypes = [I, P, P, P, I, I, P, I, P, I, P, P, P, P, ctypes.c_char_p, I]
+    lib.qasr_kernel_kv_append_planned.argtypes = [I, P, P, P, P, I, P, I, I, I, I, I, P, P, I, P, ctypes.c_char_p, I]
     lib.qasr_kernel_attention_chunk_workspace.argtypes = [I]
     lib.qasr_kernel_attention_chunk_workspace.restype = ctypes.c_int64
     lib.qasr_kernel_attention_chunk.argtypes = [I, P, I, P, I, P, I, I, P, I, P, I, I, I, I, I, I, P, P, P, I,
@@ -888,6 +889,19 @@ def kernel_kv_release(device: int, stream: int, seq_slot_ptr: int, kv_len_ptr: i
         raise DecoderError(st, buf.value.decode(errors="replace"))
 
 
+def kernel_kv_append_planned(device: int, stream: int, k_ptr: int, v_ptr: int, pool_ptr: int, pool_pages: int,
+                             page_table_ptr: int, max_slots: int, max_pages: int, layers: int, nkv: int, layer: int,
+                             row_slot_ptr: int, row_pos_ptr: int, rows_cap: int, row_count_ptr: int):
+    """Write a planned step's K and V rows into the paged cache; row_count_ptr is the plan's cu_rows + n_seqs, so a
+    refused plan writes nothing and rows behind the last one are left out."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_kv_append_planned(device, stream, k_ptr, v_ptr, pool_ptr, pool_pages, page_table_ptr, max_slots,
+                                           max_pages, layers, nkv, layer, row_slot_ptr, row_pos_ptr, rows_cap,
+                                           row_count_ptr, buf, 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
 def kernel_attention_chunk_workspace(device: int) -> int:
     """Bytes of workspace kernel_attention_chunk wants on `device` (256-byte aligned, any content)."""
     n = lib.qasr_kernel_attention_chunk_workspace(device)
@@ -968,7 +982,7 @@ def version() -> str:
 __all__ = [
     "TextDecoder", "DecoderError", "SyntheticModel", "MODEL_PRESETS", "text_config",
     "build_rope_tables", "dim_map", "kernel_pack_weights", "kernel_gemm", "kernel_attention_noalloc", "kernel_attention", "kernel_kv_append",
-    "kernel_kv_plan", "kernel_kv_release", "kernel_attention_chunk_workspace", "kernel_attention_chunk",
+    "kernel_kv_plan", "kernel_kv_release", "kernel_kv_append_planned", "kernel_attention_chunk_workspace", "kernel_attention_chunk",
     "kernel_attention_chunk_check", "kernel_w4_packed_bytes", "kernel_pack_w4", "kernel_gemv_w4", "TYPE_F16", "TYPE_BF16", "KV_PLAN_MAX_SEQS",
     "KV_PLAN_MAX_SLOTS", "W4_MAX_ROWS",
     "launch_count", "version", "WEIGHTS_F16", "WEIGHTS_INT8", "WEIGHTS_INT8_F32", "EXPORTED_SYMBOLS", "lib",

@@ -258,4 +258,40 @@ __global__ void __launch_bounds__(MAPS_THREADS) kv_row_maps_kernel(const __grid_
   }
 }
 
+// The planned step's new K and V rows, written through its maps.  Only the rows that the plan gave out are
+// written (their count is read here: a refused plan has none, and its maps are an earlier step's), and no entry of
+// the maps or of the table is followed out of its range.  A copy: each thread moves 16 bytes of K and of V.
+// Measured (B200, us in a graph, 8 kv heads): 32 rows 2.0 (a launch and a chain of three reads), 832 rows 2.5, 8192 rows 8.1
+// (67 MB, partly out of L2).
+constexpr int APPEND_THREADS = 256;
+struct AppendArgs {
+  const uint4 *k, *v;
+  uint4* pool;
+  int pool_pages;
+  const int* page_table;
+  int max_slots, max_pages, layers, nkv, layer;
+  const int *row_slot, *row_pos;
+  int rows_cap;
+  const int* row_count;
+};
+__global__ void __launch_bounds__(APPEND_THREADS) kv_append_planned_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int CHUNKS = 16;  // of 16 bytes in a row of 128
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long all = static_cast<long long>(min(a.row_count[0], a.rows_cap)) * a.nkv * CHUNKS;
+  const long long step = static_cast<long long>(gridDim.x) * APPEND_THREADS;
+  for (long long e = static_cast<long long>(blockIdx.x) * APPEND_THREADS + threadIdx.x; e < all; e += step) {
+    const long long rh = e / CHUNKS;
+    const int c = static_cast<int>(e % CHUNKS), r = static_cast<int>(rh / a.nkv), h = static_cast<int>(rh % a.nkv);
+    const int slot = a.row_slot[r], pos = a.row_pos[r];
+    if (slot < 0 || slot >= a.max_slots || pos < 0 || pos >> 6 >= a.max_pages) continue;
+    const int page = a.page_table[static_cast<size_t>(slot) * a.max_pages + (pos >> 6)];
+    if (page < 0 || page >= a.pool_pages) continue;
+    const long long k_row = (((static_cast<long long>(page) * a.layers + a.layer) * 2) * a.nkv + h) * 64 + (pos & 63);
+    const int at = c ^ (pos & 7);
+    a.pool[k_row * CHUNKS + at] = a.k[e];
+    a.pool[(k_row + static_cast<long long>(a.nkv) * 64) * CHUNKS + at] = a.v[e];
+  }
+}
+
 }  // namespace qasr

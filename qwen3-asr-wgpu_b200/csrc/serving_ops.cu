@@ -1,5 +1,5 @@
 // C entry points of the serving step over the paged cache (include/qasr_b200_kernels.h):
-// page and row maps, chunk attention, 4-bit products.  The calls check their scalar arguments,
+// page and row maps and the append through them, chunk attention, 4-bit products.  The calls check their scalar arguments,
 // enqueue on the caller's stream and return; nothing is allocated, kept or synchronised, and the
 // thread's current device is put back.
 #include <cuda.h>
@@ -250,6 +250,26 @@ qasr_status qasr_kernel_kv_release(int device, void* stream, const int* seq_slot
   PlanArgs a{seq_slot, kv_len, nullptr, n_seqs, max_slots, const_cast<int*>(page_table), max_pages, free_pages,
              pool_pages, free_count, kv_len_out, free_count_out, nullptr, nullptr, nullptr, 0, status, 0};
   return launch_plan<true>(device, stream, a, err, errlen);
+}
+
+qasr_status qasr_kernel_kv_append_planned(int device, void* stream, const uint16_t* k, const uint16_t* v, uint16_t* kv_pool,
+                                          int pool_pages, const int* page_table, int max_slots, int max_pages, int layers,
+                                          int nkv, int layer, const int* row_slot, const int* row_pos, int rows_cap,
+                                          const int* row_count, char* err, int errlen) {
+  if (!k || !v || !kv_pool || !page_table || !row_slot || !row_pos || !row_count || pool_pages <= 0 || max_slots <= 0 ||
+      max_pages <= 0 || max_pages >= (1 << 25) || layers <= 0 || layer < 0 || layer >= layers || nkv <= 0 || nkv > (1 << 20) ||
+      rows_cap <= 0 || misaligned(k, 16) || misaligned(v, 16) || misaligned(kv_pool, 16))
+    return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad planned kv append arguments");
+  DeviceScope dev(device);
+  if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
+  const int sms = sm_count(device);
+  if (sms <= 0) return op_err(err, errlen, QASR_ERR_DEVICE, "device attributes");
+  const AppendArgs a{reinterpret_cast<const uint4*>(k), reinterpret_cast<const uint4*>(v), reinterpret_cast<uint4*>(kv_pool),
+                     pool_pages, page_table, max_slots, max_pages, layers, nkv, layer, row_slot, row_pos, rows_cap, row_count};
+  const long long ctas = (static_cast<long long>(rows_cap) * nkv * 16 + APPEND_THREADS - 1) / APPEND_THREADS;
+  const cudaError_t e = launch_k(kv_append_planned_kernel, dim3(static_cast<unsigned>(std::min<long long>(ctas, sms * 8))),
+                                 dim3(APPEND_THREADS), 0, static_cast<cudaStream_t>(stream), true, a);
+  return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "planned kv append launch");
 }
 
 int64_t qasr_kernel_attention_chunk_workspace(int device) {

@@ -1,0 +1,109 @@
+"""The serving step where its operators meet: steps that are refused, and maps longer than the step's rows."""
+import random
+
+import pytest
+
+import test_gpu_serving_ops as ops
+from test_gpu_serving_ops import DIM, PAGE, Pages, _ints, _stream
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------ the append of a planned step
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("nkv,layers,layer,rows,count", [(8, 1, 0, 1, 1), (1, 3, 2, 70, 70), (5, 2, 0, 333, 200), (8, 2, 1, 40, 0),
+                                                         (8, 1, 0, 12, -3), (2, 1, 0, 9, 2**31 - 1), (8, 1, 0, 20000, 20000)])
+def test_planned_append_writes_the_rows_that_were_given_out(qasr, cuda_device, nkv, layers, layer, rows, count, dtype):
+    """Bit for bit, and nothing else: rows past the count, slots, positions and pages out of range."""
+    import torch
+    t = torch.bfloat16 if dtype == "bf16" else torch.float16
+    slots, max_pages, pool_pages = 13, 40, 600
+    rng = random.Random(rows)
+    cells = rng.sample(range(slots * max_pages * PAGE), rows)  # distinct (slot, position)
+    slot, pos = [c // (max_pages * PAGE) for c in cells], [c % (max_pages * PAGE) for c in cells]
+    for i, (s, p) in enumerate([(-1, 0), (slots, 0), (0, -1), (0, max_pages * PAGE), (2**31 - 1, 2**31 - 1)]):
+        if rows > 100:
+            slot[7 * i], pos[7 * i] = s, p
+    page = torch.randperm(pool_pages, device="cuda")[:slots * max_pages].to(torch.int32).view(slots, max_pages)
+    page[3, 5], page[4, 0], page[0, 1] = -1, pool_pages, 2**31 - 1
+    k, v = (torch.randn((rows, nkv * DIM), device="cuda").to(t) for _ in range(2))
+    pool = torch.full((pool_pages, layers, 2, nkv, PAGE, DIM), 3.0, dtype=t, device="cuda")
+    want = pool.clone()
+    m = max(0, min(count, rows))
+    s, p = (torch.tensor(x[:m], dtype=torch.int64, device="cuda") for x in (slot, pos))
+    ok = (s >= 0) & (s < slots) & (p >= 0) & (p < max_pages * PAGE)
+    s, p, kk, vv = s[ok], p[ok], k[:m][ok], v[:m][ok]
+    pg = page[s, p // PAGE].long()
+    ok = (pg >= 0) & (pg < pool_pages)
+    pg, p, kk, vv = pg[ok], p[ok], kk[ok], vv[ok]
+    d = torch.arange(DIM, device="cuda")
+    col = (((d >> 3)[None, :] ^ (p & 7)[:, None]) << 3) | (d & 7)[None, :]
+    for h in range(nkv):
+        for part, x in enumerate((kk, vv)):
+            want[pg[:, None], layer, part, h, (p % PAGE)[:, None], col] = x[:, h * DIM:(h + 1) * DIM]
+    d_slot, d_pos, d_count = _ints(slot, torch), _ints(pos, torch), _ints([count], torch)
+    qasr.kernel_kv_append_planned(0, _stream(torch), k.data_ptr(), v.data_ptr(), pool.data_ptr(), pool_pages, page.data_ptr(),
+                                  slots, max_pages, layers, nkv, layer, d_slot.data_ptr(), d_pos.data_ptr(), rows,
+                                  d_count.data_ptr())
+    torch.cuda.synchronize()
+    assert torch.equal(pool, want)
+
+
+@pytest.mark.parametrize("rows_cap", [3, 8, 60000])  # exact maps, longer ones, maps that a second kernel writes
+def test_a_captured_step_that_runs_out_of_pages_leaves_the_cache_alone(qasr, cuda_device, rows_cap):
+    """Plan, append and attention in one graph, replayed until the free stack is empty: the refused step writes nothing, in
+    spite of the maps that still hold the step before, and the steps before it only their own rows."""
+    import torch
+    n, slots, max_pages, pool_pages, nkv, nq = 3, 5, 4, 4, 8, 16
+    p = Pages(torch, slots, max_pages, pool_pages, seed=3)
+    slot, held = [4, 1, 2], [62, 20, 64]
+    ops._check_plan(p, p.plan(qasr, slot, [0] * n, held), slot, [0] * n, held)
+    d_slot, d_len, cu, status = _ints(slot, torch), _ints(held, torch), _ints([0] * (n + 1), torch), _ints([-9, -9], torch)
+    # before the first step the maps are whatever the memory held
+    maps = [torch.randint(-2**31, 2**31 - 1, (rows_cap,), dtype=torch.int32, device="cuda") for _ in range(2)]
+    pool = torch.randn((pool_pages, 1, 2, nkv, PAGE, DIM), device="cuda").to(torch.float16)
+    k, v = (torch.randn((rows_cap, nkv * DIM), device="cuda").to(torch.float16) for _ in range(2))
+    q = torch.randn((rows_cap, nq * DIM), device="cuda").to(torch.float16)
+    out = torch.full_like(q, 77)
+    ws_bytes = qasr.kernel_attention_chunk_workspace(0)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
+
+    def step():
+        st = _stream(torch)
+        qasr.kernel_kv_plan(0, st, d_slot.data_ptr(), d_len.data_ptr(), None, n, slots, p.d_table.data_ptr(), max_pages,
+                            p.d_free.data_ptr(), pool_pages, p.d_count.data_ptr(), d_len.data_ptr(), p.d_count.data_ptr(),
+                            cu.data_ptr(), maps[0].data_ptr(), maps[1].data_ptr(), rows_cap, status.data_ptr())
+        qasr.kernel_kv_append_planned(0, st, k.data_ptr(), v.data_ptr(), pool.data_ptr(), pool_pages, p.d_table.data_ptr(),
+                                      slots, max_pages, 1, nkv, 0, maps[0].data_ptr(), maps[1].data_ptr(), rows_cap,
+                                      cu.data_ptr() + 4 * n)
+        qasr.kernel_attention_chunk(0, st, qasr.TYPE_F16, q.data_ptr(), nq * DIM, out.data_ptr(), nq * DIM, rows_cap,
+                                    pool.data_ptr(), pool_pages, p.d_table.data_ptr(), slots, max_pages, 1, nq, nkv, 0,
+                                    d_slot.data_ptr(), cu.data_ptr(), d_len.data_ptr(), n, ws.data_ptr(), ws_bytes)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    # one page is left, taken by the third request's first step; the first request wants another one in its third
+    for i, refused in enumerate([False, False, True, True]):
+        for x in (k, v, q):
+            x.copy_(torch.randn_like(x))
+        out.fill_(77)
+        before = pool.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        if refused:
+            assert status.tolist() == [3, -1] and d_len.tolist() == held and cu.tolist() == [0] * (n + 1)
+            assert torch.equal(pool, before) and (out == 77).all()
+            continue
+        p.expect(slot, held, [1] * n)
+        assert status.tolist() == [0, 0] and p.d_table.tolist() == p.table
+        for r, (s, pos) in enumerate(zip(slot, held)):
+            d = torch.arange(DIM, device="cuda")
+            col = (((d >> 3) ^ (pos & 7)) << 3) | (d & 7)
+            for part, x in enumerate((k, v)):
+                before[p.table[s][pos // PAGE], 0, part, :, pos % PAGE, col] = x[r].view(nkv, DIM)
+        held = [h + 1 for h in held]
+        assert torch.equal(pool, before) and d_len.tolist() == held
+        assert out[:n].isfinite().all() and (out[:n] != 77).any() and (out[n:] == 77).all()
