@@ -239,10 +239,14 @@ qasr_status qasr_kernel_pack_w4(int device, void* stream, const uint8_t* codes, 
  * for 1 <= rows <= QASR_W4_MAX_ROWS; x [rows, ldx], out [rows, ldo] of `type`, ldx >= k a multiple
  * of 8, ldo >= n_out, x on a 16-byte boundary; out may overlap neither x nor packed.  Codes and zero
  * points enter the product exactly, each group's sum and the sum over groups are f32.
- * Only enqueues: a bounded device-side wait for its own copies that gives up is not reported. */
+ * Only enqueues.  If a bounded device-side wait for its own copies gives up, the outputs whose sums lack a
+ * part are NaN, and qasr_kernel_gemv_w4_check tells. */
 qasr_status qasr_kernel_gemv_w4(int device, void* stream, int type, const void* packed, int has_zero,
                                 int n_out, int k, int group, const void* x, int ldx, int rows, void* out,
                                 int ldo, int accumulate, char* err, int errlen);
+/* Waits for `stream`; QASR_ERR_DEVICE_TIMEOUT if a wait of any qasr_kernel_gemv_w4 on `device` gave up since
+ * this was last asked (one word per device, whatever the stream: only the first to ask is told). */
+qasr_status qasr_kernel_gemv_w4_check(int device, void* stream, char* err, int errlen);
 
 /* Number of kernels this library launched since load (all contexts and probes). */
 uint64_t qasr_kernel_launch_count(void);

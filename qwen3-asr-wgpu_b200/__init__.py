@@ -63,6 +63,7 @@ EXPORTED_SYMBOLS = (
     "qasr_kernel_launch_count",
     "qasr_kernel_kv_plan", "qasr_kernel_kv_release", "qasr_kernel_kv_append_planned", "qasr_kernel_attention_chunk_workspace",
     "qasr_kernel_attention_chunk", "qasr_kernel_attention_chunk_check", "qasr_kernel_w4_packed_bytes", "qasr_kernel_pack_w4", "qasr_kernel_gemv_w4",
+    "qasr_kernel_gemv_w4_check",
     "qasr_synth_key", "qasr_synth_normal_f16", "qasr_synth_uniform_ids",
     "qasr_synth_quantize_rows", "qasr_f32_to_f16", "qasr_f16_to_f32", "qasr_f32_to_f16_array",
     "qasr_f16_to_f32_array",
@@ -284,6 +285,7 @@ def _load() -> ctypes.CDLL:
     lib.qasr_kernel_w4_packed_bytes.restype = ctypes.c_int64
     lib.qasr_kernel_pack_w4.argtypes = [I, P, P, P, P, I, I, I, P, ctypes.c_char_p, I]
     lib.qasr_kernel_gemv_w4.argtypes = [I, P, I, P, I, I, I, I, P, I, I, P, I, I, ctypes.c_char_p, I]
+    lib.qasr_kernel_gemv_w4_check.argtypes = [I, P, ctypes.c_char_p, I]
     lib.qasr_synth_key.argtypes = [ctypes.c_uint64, ctypes.c_uint64]
     lib.qasr_synth_key.restype = ctypes.c_uint64
     lib.qasr_synth_normal_f16.argtypes = [P, ctypes.c_size_t, ctypes.c_uint64, ctypes.c_uint64,
@@ -960,6 +962,14 @@ def kernel_gemv_w4(device: int, stream: int, type: int, packed_ptr: int, has_zer
         raise DecoderError(st, buf.value.decode(errors="replace"))
 
 
+def kernel_gemv_w4_check(device: int, stream: int):
+    """Wait for the stream; raise if a device-side wait of a kernel_gemv_w4 on the device gave up since the last check."""
+    buf = _op_buf()
+    st = lib.qasr_kernel_gemv_w4_check(device, stream, buf, 512)
+    if st != QASR_OK:
+        raise DecoderError(st, buf.value.decode(errors="replace"))
+
+
 def kv_page_swizzle(pool: np.ndarray) -> np.ndarray:
     """Convert KV pool pages [..., 64, 128] between the logical row layout and the
     swizzled one the kernels use (dim d of position p at column ((d // 8) ^ (p % 8)) * 8
@@ -983,7 +993,7 @@ __all__ = [
     "TextDecoder", "DecoderError", "SyntheticModel", "MODEL_PRESETS", "text_config",
     "build_rope_tables", "dim_map", "kernel_pack_weights", "kernel_gemm", "kernel_attention_noalloc", "kernel_attention", "kernel_kv_append",
     "kernel_kv_plan", "kernel_kv_release", "kernel_kv_append_planned", "kernel_attention_chunk_workspace", "kernel_attention_chunk",
-    "kernel_attention_chunk_check", "kernel_w4_packed_bytes", "kernel_pack_w4", "kernel_gemv_w4", "TYPE_F16", "TYPE_BF16", "KV_PLAN_MAX_SEQS",
+    "kernel_attention_chunk_check", "kernel_w4_packed_bytes", "kernel_pack_w4", "kernel_gemv_w4", "kernel_gemv_w4_check", "TYPE_F16", "TYPE_BF16", "KV_PLAN_MAX_SEQS",
     "KV_PLAN_MAX_SLOTS", "W4_MAX_ROWS",
     "launch_count", "version", "WEIGHTS_F16", "WEIGHTS_INT8", "WEIGHTS_INT8_F32", "EXPORTED_SYMBOLS", "lib",
     "Checkpoint", "read_model_config", "ModelConfig", "batch_decode_backend", "STOP_EOS", "STOP_MAX_TOKENS",

@@ -170,6 +170,7 @@ struct W4Type<true> {
 // is what comes closest to the memory's pace.  Measured (B200, us in a graph): 151936 x 2048 at one row 34.5 (4.7 TB/s), 60000
 // x 8192 at one row 49.9 (5.1 TB/s, 78% of the measured copy rate), at 16 rows 76, at 32 rows 150 (there x's way from
 // L1 and the matrix instructions bound it), 2048 x 6144 at one row 4.4, 1024 x 2048 2.7 (latency).
+// A wait for a copy that gives up is recorded in w4_status, and every output whose sum then lacks a part is NaN.
 constexpr int W4_WARPS = 8;
 constexpr int W4_THREADS = W4_WARPS * 32;
 constexpr int W4_MAX_CLUSTER = 4;
@@ -187,7 +188,19 @@ struct W4Plan {
   static constexpr int smem = bars_bytes + slots * W4_WARPS * unit_bytes + sums_bytes;
 };
 
-template <bool BF16, bool ZERO, int GS, int NT>
+// {error, site} of the first wait that gave up since the words were last read (report_error).
+static __device__ uint32_t w4_status[2];
+constexpr uint32_t W4_WAIT_SITE = 0x40;
+
+// How a unit comes into its slot (a test loses one here).
+struct W4Copy {
+  static __device__ __forceinline__ void unit(void* slot, const uint8_t* from, uint32_t bytes, uint64_t* full, int /*tile*/, int /*unit*/) {
+    mbar_arrive_expect_tx(full, bytes);
+    bulk_load(slot, from, bytes, full);
+  }
+};
+
+template <bool BF16, bool ZERO, int GS, int NT, class COPY = W4Copy>
 __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) gemv_w4_kernel(const __grid_constant__ W4Args a) {
   using TT = W4Type<BF16>;
   using T = typename TT::T;
@@ -226,8 +239,7 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
   };
   auto copy_next = [&](int slot) {  // lane 0
     if (cg >= groups) return;
-    mbar_arrive_expect_tx(&full[slot], P::unit_bytes);
-    bulk_load(ring + slot * P::unit_bytes, from, P::unit_bytes, &full[slot]);
+    COPY::unit(ring + slot * P::unit_bytes, from, P::unit_bytes, &full[slot], cg * wt_n + wt, cu);
     cu += wk_n;
     from += stride;
     if (cu >= u1) {
@@ -331,7 +343,7 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
         for (int u = u0; u < u1 && !lost; u += wk_n) {
           if constexpr (PRE) fetch_x(u);
           if (!__all_sync(0xffffffffu, mbar_try_wait(&full[slot], parity)) &&
-              !mbar_wait_warp(&full[slot], parity, abort_flag, nullptr, 0)) {
+              !mbar_wait_warp(&full[slot], parity, abort_flag, w4_status, W4_WAIT_SITE)) {
             lost = true;
             break;
           }
@@ -353,7 +365,8 @@ __global__ void __launch_bounds__(W4_THREADS, (W4Plan<ZERO, GS, NT>::per_sm)) ge
         for (int m = 0; m < NT; ++m)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            mysums[(m * 8 + t * 2 + (c & 1)) * 33 + i * 16 + (lane >> 2) + (c >> 1) * 8] = acc[i][m][c];
+            mysums[(m * 8 + t * 2 + (c & 1)) * 33 + i * 16 + (lane >> 2) + (c >> 1) * 8] =
+                lost ? __uint_as_float(0x7fffffffu) : acc[i][m][c];  // NaN: the sum lacks this warp's part, or some of it
       __syncthreads();
       for (int e = tid; e < a.rows * 32 * wt_n; e += W4_THREADS) {
         const int c = e % (32 * wt_n), r = e / (32 * wt_n);

@@ -383,4 +383,17 @@ qasr_status qasr_kernel_gemv_w4(int device, void* stream, int type, const void* 
   return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "w4 gemv launch");
 }
 
+qasr_status qasr_kernel_gemv_w4_check(int device, void* stream, char* err, int errlen) {
+  DeviceScope dev(device);
+  if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint32_t got[2] = {0, 0}, none[2] = {0, 0};
+  cudaError_t e = cudaMemcpyFromSymbolAsync(got, w4_status, sizeof got, 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && got[0]) e = cudaMemcpyToSymbolAsync(w4_status, none, sizeof none, 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess && got[0]) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return op_cuda(err, errlen, e, "w4 gemv status");
+  return got[0] ? op_err(err, errlen, QASR_ERR_DEVICE_TIMEOUT, "a device-side wait of a w4 gemv timed out") : QASR_OK;
+}
+
 }  // extern "C"
