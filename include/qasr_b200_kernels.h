@@ -215,10 +215,10 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
                                         const int* seq_slot, const int* cu_rows, const int* kv_len,
                                         int n_seqs, float scale, void* ws, int64_t ws_bytes, char* err,
                                         int errlen);
-/* Waits for `stream` and tells how the last qasr_kernel_attention_chunk over `ws` went:
- * QASR_ERR_DEVICE_TIMEOUT if a bounded device-side wait gave up (its output is then not to be used). */
-qasr_status qasr_kernel_attention_chunk_check(int device, void* stream, const void* ws, char* err,
-                                              int errlen);
+/* Waits for `stream`; QASR_ERR_DEVICE_TIMEOUT if a bounded device-side wait of any qasr_kernel_attention_chunk over `ws`
+ * gave up since this was last asked (the outputs of such a call are not to be used).  Calls leave a mark in ws
+ * that later calls keep and this one clears, so once after all layers, or after several steps, is enough. */
+qasr_status qasr_kernel_attention_chunk_check(int device, void* stream, void* ws, char* err, int errlen);
 
 #define QASR_W4_MAX_ROWS 64
 

@@ -928,7 +928,7 @@ def kernel_attention_chunk(device: int, stream: int, type: int, q_ptr: int, q_ld
 
 
 def kernel_attention_chunk_check(device: int, stream: int, ws_ptr: int):
-    """Wait for the stream; raise if a device-side wait of the last kernel_attention_chunk over ws gave up."""
+    """Wait for the stream; raise if a device-side wait of any kernel_attention_chunk over ws gave up since the last check."""
     buf = _op_buf()
     st = lib.qasr_kernel_attention_chunk_check(device, stream, ws_ptr, buf, 512)
     if st != QASR_OK:

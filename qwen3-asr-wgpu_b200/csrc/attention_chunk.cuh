@@ -97,7 +97,11 @@ struct ChunkMeta {
   int state;  // 1: it began such a block; 2: a wait gave up
   int row0, ntok, head, pos0;
   int went_on;  // 1: it went on with the block of the CTAs before it; 2: and finished it
+  int unused[2];
+  uint32_t lost[4];  // chunk_lost(0..3) once a wait of any call has given up: no call clears it, only the check does
 };
+// Four words that a workspace of arbitrary content does not hold by chance.
+__host__ __device__ constexpr uint32_t chunk_lost(int i) { return 0x6c6f7374u * (2 * i + 1) + 0x9e3779b9u; }
 __host__ __device__ constexpr long long chunk_meta_bytes(int grid) { return (grid * 64ll + 255) / 256 * 256; }
 __host__ __device__ constexpr long long chunk_ws_bytes(int grid) {
   return chunk_meta_bytes(grid) + 2ll * grid * CHUNK_PART_FLOATS * 4;
@@ -1109,7 +1113,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (tid == 0 && B.abort_flag) meta->state = 2;
+  if (tid == 0 && B.abort_flag) {
+    meta->state = 2;
+    for (int i = 0; i < 4; ++i) meta->lost[i] = chunk_lost(i);
+  }
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 

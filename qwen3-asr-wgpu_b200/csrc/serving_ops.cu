@@ -7,6 +7,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <cstddef>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -330,7 +331,7 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
   return e == cudaSuccess ? QASR_OK : op_cuda(err, errlen, e, "chunk attention combine launch");
 }
 
-qasr_status qasr_kernel_attention_chunk_check(int device, void* stream, const void* ws, char* err, int errlen) {
+qasr_status qasr_kernel_attention_chunk_check(int device, void* stream, void* ws, char* err, int errlen) {
   if (!ws || misaligned(ws, 256)) return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad chunk attention workspace");
   DeviceScope dev(device);
   if (dev.error != cudaSuccess) return op_cuda(err, errlen, dev.error, "device");
@@ -342,12 +343,17 @@ qasr_status qasr_kernel_attention_chunk_check(int device, void* stream, const vo
   cudaError_t e = cudaMemcpyAsync(lines, ws, static_cast<size_t>(grid) * 64, cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e != cudaSuccess) return op_cuda(err, errlen, e, "chunk attention status");
+  bool lost = false;
   for (int c = 0; c < grid; ++c) {
-    int state;
-    std::memcpy(&state, lines + c * 64, sizeof state);
-    if (state == 2) return op_err(err, errlen, QASR_ERR_DEVICE_TIMEOUT, "a device-side wait of the chunk attention timed out");
+    ChunkMeta m;
+    std::memcpy(&m, lines + c * 64, sizeof m);
+    lost |= m.lost[0] == chunk_lost(0) && m.lost[1] == chunk_lost(1) && m.lost[2] == chunk_lost(2) && m.lost[3] == chunk_lost(3);
   }
-  return QASR_OK;
+  if (!lost) return QASR_OK;
+  e = cudaMemset2DAsync(static_cast<uint8_t*>(ws) + offsetof(ChunkMeta, lost), 64, 0, sizeof ChunkMeta::lost, grid, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return op_cuda(err, errlen, e, "chunk attention status");
+  return op_err(err, errlen, QASR_ERR_DEVICE_TIMEOUT, "a device-side wait of the chunk attention timed out");
 }
 
 int64_t qasr_kernel_w4_packed_bytes(int n_out, int k, int group, int has_zero) {

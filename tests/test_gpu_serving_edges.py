@@ -107,3 +107,33 @@ def test_a_captured_step_that_runs_out_of_pages_leaves_the_cache_alone(qasr, cud
         held = [h + 1 for h in held]
         assert torch.equal(pool, before) and d_len.tolist() == held
         assert out[:n].isfinite().all() and (out[:n] != 77).any() and (out[n:] == 77).all()
+
+
+# ------------------------------------------------------------------------------------ waits that gave up
+@pytest.mark.parametrize("cta", [0, 77, -1])
+def test_a_wait_that_gave_up_is_told_however_many_calls_follow(qasr, cuda_device, cta):
+    """The mark that a call leaves in its CTA's line of the workspace (written here from the host, four words from byte
+    32 on) outlives the calls after it, eager and captured, until the check has told it once."""
+    import torch
+    c = ops.Chunks(torch, [(700, 90), (1200, 1), (0, 300)], seed=30)
+    ws = c.workspace(qasr)
+    c.run(qasr, ws=ws)
+    qasr.kernel_attention_chunk_check(0, _stream(torch), ws[0].data_ptr())
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    mark = torch.tensor([(0x6c6f7374 * (2 * i + 1) + 0x9e3779b9) % 2**32 for i in range(4)], dtype=torch.uint32, device="cuda")
+    ws[0].view(torch.uint32)[:16 * sms].view(sms, 16)[cta, 8:12] = mark
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        c.run(qasr, ws=ws)
+    for _ in range(3):
+        c.run(qasr, ws=ws)
+        graph.replay()
+    with pytest.raises(qasr.DecoderError) as e:
+        qasr.kernel_attention_chunk_check(0, _stream(torch), ws[0].data_ptr())
+    assert e.value.status == 5
+    qasr.kernel_attention_chunk_check(0, _stream(torch), ws[0].data_ptr())
+    c.run(qasr, ws=ws)
+    qasr.kernel_attention_chunk_check(0, _stream(torch), ws[0].data_ptr())
+    c.check(c.out)
