@@ -345,10 +345,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 2^x for two x <= 2^8 on the FMA pipe: x = n + f with n the nearest integer, 2^f by the polynomial of degree 4 with the
+// 2^x for two x <= CHUNK_RESCALE (right for any x < 127.5) on the FMA pipe: x = n + f with n the nearest integer, 2^f by the polynomial of degree 4 with the
 // smallest largest relative error on [-1/2, 1/2] and value 1 at 0 (2.9e-6 in f32, found by weighted least squares; f16 rounds P
 // to 4.9e-4), n added to the exponent.  At -127 and below, a masked score's -inf among them, the result is exactly 0.  What is
-// not a number becomes 2^128 or more once rounded, so the row comes out not finite and is computed again (chunk_row).
+// not a number becomes the largest f32: P rounds it to infinity, and the sum shows it (2^127 and more).
+static_assert(CHUNK_RESCALE < 15.0f, "P, up to 2^CHUNK_RESCALE, is finite in f16, and ex2_poly2 has no overflow to handle");
 __device__ __forceinline__ void ex2_poly2(uint64_t x2, float& a, float& b) {
   float xa, xb;
   unpack2(x2, xa, xb);
@@ -665,7 +666,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&B.p_full[grp][n_tile & 1]);
       }
-      if (l != l) m = l;  // a score that is not a number must show in every join
+      // A score that is not a number must show in every join.  ex2_poly2 makes 2^128 of it, which no sum of real
+      // probabilities reaches (each is at most 2^CHUNK_RESCALE), and m may be -inf beside it: a maximum passes over it.
+      if (!(l < 0x1p127f)) m = l = __uint_as_float(0x7fffffffu);
       // ---- the block's end
       const bool had = first < count;  // this group had tiles
       if (had) {

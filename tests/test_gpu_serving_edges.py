@@ -137,3 +137,22 @@ def test_a_wait_that_gave_up_is_told_however_many_calls_follow(qasr, cuda_device
     c.run(qasr, ws=ws)
     qasr.kernel_attention_chunk_check(0, _stream(torch), ws[0].data_ptr())
     c.check(c.out)
+
+
+# ------------------------------------------------------------------------------------ scores that are not numbers
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("at", [0, 5, 6, 7, 14, 15, 62, 63, 64 + 6, 128 + 31])
+def test_a_key_that_is_not_a_number_among_keys_of_minus_infinity(qasr, cuda_device, at, dtype):
+    """One NaN key, every other key of the first 1024 positions so low that its score is -inf: the running maximum passes
+    over both.  Every row that sees the NaN is NaN, in a prompt, a short chunk, a whole decode row and one whose keys
+    are cut over CTAs, the other parts of which are finite; rows before it are NaN too, softmax of nothing but -inf."""
+    import torch
+    c = ops.Chunks(torch, [(0, 200), (160, 20), (250, 1), (9000, 1)], seed=31, dtype=dtype)
+    c.q.abs_().add_(0.01)
+    for kv in c.kv:
+        kv[0, :, :1024] = -float("inf")
+        kv[0, :, at] = float("nan")
+    c.store()
+    out = c.run(qasr)
+    torch.cuda.synchronize()
+    assert out[:222, :2048].isnan().all()
