@@ -194,7 +194,7 @@ qasr_status qasr_kernel_kv_append_planned(int device, void* stream, const uint16
  * A row at p < 0 sees nothing and is written as zeros; rows that no request owns are left as they
  * were.  Chunks of any length go into one call: a decode step is n = 1 everywhere.
  * type: QASR_TYPE_F16 or QASR_TYPE_BF16, of q, out and the cache.  q [rows, q_ld], out [rows,
- * out_ld]: q_ld, out_ld >= nq * 128 and multiples of 8, both pointers and kv_pool on 16-byte
+ * out_ld], |scale| < 2^127: q_ld, out_ld >= nq * 128 and multiples of 8, both pointers and kv_pool on 16-byte
  * boundaries; out may not overlap q.  nq a multiple of nkv, nq / nkv <= 16.  kv_pool
  * [pool_pages][layers][2][nkv][64][128] in the layout of qasr_kernel_attention; at most 2^31 - 1
  * rows of 128.  page_table [max_slots][max_pages], max_pages < 2^25.

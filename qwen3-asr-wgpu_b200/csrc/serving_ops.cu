@@ -287,7 +287,7 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
       pool_pages <= 0 || max_slots <= 0 || max_pages <= 0 || max_pages >= (1 << 25) || layers <= 0 || layer < 0 ||
       layer >= layers || nkv <= 0 || nq <= 0 || nq % nkv != 0 || nq / nkv > 16 || nq > (1 << 20) ||
       q_ld < nq * CHUNK_DIM || out_ld < nq * CHUNK_DIM || q_ld % 8 || out_ld % 8 || misaligned(q, 16) ||
-      misaligned(out, 16) || misaligned(kv_pool, 16) || misaligned(ws, 256) || !std::isfinite(scale) ||
+      misaligned(out, 16) || misaligned(kv_pool, 16) || misaligned(ws, 256) || !(std::fabs(scale) < 0x1p127f) ||
       (type != QASR_TYPE_F16 && type != QASR_TYPE_BF16) ||
       static_cast<__int128>(pool_pages) * layers * 2 * nkv * CHUNK_PAGE > 0x7fffffff)
     return op_err(err, errlen, QASR_ERR_INVALID_ARG, "bad chunk attention arguments");
@@ -314,8 +314,9 @@ qasr_status qasr_kernel_attention_chunk(int device, void* stream, int type, cons
   if (!encode_map(&q_big, q, 4, q_dims, q_strides, big, true) || !encode_map(&q_small, q, 4, q_dims, q_strides, small, true) ||
       !encode_map(&kv_map, kv_pool, 3, kv_dims, kv_strides, kv_box, false))
     return op_err(err, errlen, QASR_ERR_DEVICE, "chunk attention tensor maps");
-  // a scale of 0 becomes a tiny one: masked scores stay -inf under it, and every other score still counts alike
-  const float s2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+  // A scale of 0 becomes the smallest number: masked scores stay -inf under it, and no finite score moves a probability
+  // by more than 2^-20 (2^128 * 2^-149).
+  const float s2 = scale == 0.0f ? 0x1p-149f : std::fabs(scale) * 1.4426950408889634f;
   const ChunkArgs a{q, q_ld, out, out_ld, rows, kv_pool, pool_pages, page_table, max_slots, max_pages, layers, nq, nkv,
                     layer, group, chunk_tile_tokens(group), seq_slot, cu_rows, kv_len, n_seqs, s2, scale < 0.0f, static_cast<uint8_t*>(ws)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -156,3 +156,19 @@ def test_a_key_that_is_not_a_number_among_keys_of_minus_infinity(qasr, cuda_devi
     out = c.run(qasr)
     torch.cuda.synchronize()
     assert out[:222, :2048].isnan().all()
+
+
+# ------------------------------------------------------------------------------------ scales
+@pytest.mark.parametrize("scale,size", [(1e-33, 1e16), (-1e-33, 1e16), (1e-37, 1e18), (0.0, 1e18), (0.0, 1.0), (1e-30, 1e15),
+                                        (1e20, 1e-10), (1.5e38, 0.0)])
+def test_chunk_attention_takes_scales_of_any_size(qasr, cuda_device, scale, size):
+    """Tiny scales under huge scores, 0 among them, and the other way round (bf16 has the range for it)."""
+    import torch
+    c = ops.Chunks(torch, [(0, 100), (300, 1), (64, 64)], seed=32, dtype="bf16")
+    c.q *= size
+    for kv in c.kv:
+        kv[0] *= size
+    c.store()
+    out = c.run(qasr, scale=scale)
+    torch.cuda.synchronize()
+    c.check(out, scale=scale)

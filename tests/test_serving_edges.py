@@ -51,3 +51,11 @@ def test_the_polynomial_that_takes_a_share_of_the_exponentials():
     assert np.max(np.abs(ex2(x) - want) / want) < 2.9e-6 + 4 * 2.0 ** -24
     assert ex2(np.zeros(1, f32))[0] == 1
     assert (ex2(np.array([-127, -128, -1e30, -np.inf], f32)) == 0).all()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, -(2.0 ** 127), 3.4e38, float("inf"), float("nan")])
+def test_attention_chunk_refuses_scales_that_leave_f32(qasr, scale):
+    """The softmax runs in powers of two, under scale * log2(e)."""
+    with pytest.raises(qasr.DecoderError) as e:
+        qasr.kernel_attention_chunk(0, 0, 0, A, 2048, A, 2048, 5, A, 9, A, 4, 8, 2, 16, 8, 1, A, A, A, 2, A, 1 << 40, scale=scale)
+    assert e.value.status == 1 and "chunk attention" in str(e.value)
