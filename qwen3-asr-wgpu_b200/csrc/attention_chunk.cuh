@@ -42,8 +42,9 @@
 //
 // Masked keys: S is replaced, never added to, so whatever stands there cannot matter; their P is 0, and
 // V rows behind the block's last position are zeroed in shared memory, so that 0 * NaN cannot arise.  What remains
-// is a V that is not finite at a position which later rows of the same block may see and earlier ones may not: a row
-// whose result is not finite is computed again without matrix instructions (chunk_row).
+// is a V that is not finite at a position which later rows of the same block may see and earlier ones may not, or an
+// infinite one under a P that was rounded to 0: a row that is not finite, and not because of what it may see, is
+// computed again without matrix instructions (chunk_row).
 #pragma once
 #include <cuda_bf16.h>
 #include "device_common.cuh"
@@ -86,7 +87,7 @@ constexpr int CHUNK_SMEM = CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * C
 constexpr int CHUNK_BLOCK_COST = 4;               // a block's Q copy, first and last steps, in key tiles (2: 32 slots 33.7 us, 4: 30.9, 6: 31.6)
 constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
-constexpr uint32_t CHUNK_WAIT_STEPS = (10 * QASR_WAIT_NS) >> 20;  // rows computed again by chunk_row keep the others waiting
+constexpr uint32_t CHUNK_WAIT_STEPS = (10 * QASR_WAIT_NS) >> 20;  // chunk_row keeps the others waiting: 2.6 s for 32 rows of 2^20 positions
 constexpr int CHUNK_PART_ROWS = 256;
 constexpr int CHUNK_PART_LD = CHUNK_DIM + 4;                     // a row's o, m, l
 constexpr int CHUNK_PART_FLOATS = CHUNK_PART_LD * CHUNK_PART_ROWS;
@@ -423,45 +424,107 @@ __device__ __forceinline__ bool chunk_wait_one(uint64_t* bar, uint32_t parity, v
   return true;
 }
 
-// One row's (m, l, o) over the positions [t0, t1) without matrix instructions: a warp, lane l holding the dims
-// 4l .. 4l + 3.  For the rows whose tensor core result is not finite.
+// A row whose tensor core result is not finite, over the positions [t0, t1), by a warp whose lane l holds the dims 4l .. 4l + 3 (and
+// leaves them alone unless `mine`).  Done as soon as what the row sees explains it: a NaN where a V is NaN, an infinity where one
+// is infinite.  Else the row is computed without matrix instructions, into `part` (under the maximum r_m that stands
+// there) or, where that is null, the output.  32 positions at a time (of one page), their loads under way together, since
+// latency is what this takes.  For the scores a lane holds the dims of chunk l % 16 of 16 positions, whose sums over the lanes are
+// exchanged so that each lane ends up with its own position's.
+// (ms, 2048 rows from nothing, all finite 0.055: a V that is not finite at position 0, seen by all, 0.37; one at the end, seen by the
+// last rows only and computed again for the others of the last block, 5.1.)
 template <bool BF16>
-__device__ __noinline__ void chunk_row(const ChunkArgs& a, int slot, int row, int qhead, int t0, int t1,
-                                       float& m, float& l, float4& o) {
+__device__ __noinline__ void chunk_row(const ChunkArgs& a, int slot, int row, int qhead, int t0, int t1, bool mine, float* part,
+                                       float r_m) {
   using TT = ChunkType<BF16>;
   using T = typename TT::T;
-  const int lane = threadIdx.x & 31, head = qhead / a.group;
-  const uint2 qv = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) + static_cast<size_t>(row) * a.q_ld +
-                                                   qhead * CHUNK_DIM + lane * 4);
-  const float2 q01 = TT::to_f32(qv.x), q23 = TT::to_f32(qv.y);
-  m = -INFINITY;
-  l = 0.0f;
-  o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int t = t0; t < t1; ++t) {
-    const long long kr = chunk_kv_row(a, slot, t, 0, head), vr = chunk_kv_row(a, slot, t, 1, head);
-    const int at = (((lane >> 1) ^ (t & 7)) << 3) + (lane & 1) * 4;
-    uint2 kv = {}, vv = {};
-    if (kr >= 0) {
-      kv = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.pool) + kr * CHUNK_DIM + at);
-      vv = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.pool) + vr * CHUNK_DIM + at);
-    }
-    const float2 k01 = TT::to_f32(kv.x), k23 = TT::to_f32(kv.y);
-    float d = q01.x * k01.x + q01.y * k01.y + q23.x * k23.x + q23.y * k23.y;
+  const int lane = threadIdx.x & 31, chunk = lane & 15, upper = lane & 16, head = qhead / a.group;
+  const float scale = a.negate ? -a.scale_log2 : a.scale_log2;
+  const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<size_t>(row) * a.q_ld + qhead * CHUNK_DIM + chunk * 8);
+  auto dot = [](uint4 x, uint4 y) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+    float d = 0.0f;
 #pragma unroll
-    for (int x = 16; x; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-    d *= a.negate ? -a.scale_log2 : a.scale_log2;
-    const float m2 = fmaxf(m, d);
-    const float base = m2 == -INFINITY ? 0.0f : m2;
-    const float f = ex2(m - base), p = ex2(d - base);
-    const float2 v01 = TT::to_f32(vv.x), v23 = TT::to_f32(vv.y);
-    l = l * f + p;
-    o.x = o.x * f + p * v01.x;
-    o.y = o.y * f + p * v01.y;
-    o.z = o.z * f + p * v23.x;
-    o.w = o.w * f + p * v23.y;
-    m = m2;
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = TT::to_f32(u[i]), g = TT::to_f32(v[i]);
+      d = fmaf(f.x, g.x, fmaf(f.y, g.y, d));
+    }
+    return d;
+  };
+  unsigned want = 0, seen = 0;  // bits x, 4 + x: dim x is NaN, is infinite; a V there is
+  auto kind = [](float f, int x) { return fabsf(f) < INFINITY ? 0u : f != f ? 1u << x : 16u << x; };
+  float4* part_at = reinterpret_cast<float4*>(part) + lane;
+  uint2* out_at = reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_ld + qhead * CHUNK_DIM) + lane;
+  if (mine) {
+    float4 was;
+    if (part) {
+      was = *part_at;
+    } else {
+      const float2 w01 = TT::to_f32(out_at->x), w23 = TT::to_f32(out_at->y);
+      was = make_float4(w01.x, w01.y, w23.x, w23.y);
+    }
+    want = kind(was.x, 0) | kind(was.y, 1) | kind(was.z, 2) | kind(was.w, 3);
   }
-  if (l != l) m = l;  // a score that is not a number: what joins this with other ranges must see it
+  float m = -INFINITY, l = 0.0f;  // l: of this lane's positions
+  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = t0; t < t1; t += 32) {
+    const int n = min(32, t1 - t);
+    const long long k_row = chunk_kv_row(a, slot, t, 0, head), v_row = k_row + static_cast<long long>(a.nkv) * CHUNK_PAGE;
+    const T* k = static_cast<const T*>(a.pool) + k_row * CHUNK_DIM;
+    const T* v = static_cast<const T*>(a.pool) + v_row * CHUNK_DIM + (lane & 1) * 4;
+    uint4 kw[16];
+    uint2 vw[16];
+#pragma unroll
+    for (int y = 0; y < 16; ++y)  // (a page out of the pool reads as zeros)
+      kw[y] = k_row < 0 || y + upper >= n ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(k + (y + upper) * CHUNK_DIM + (chunk ^ (y & 7)) * 8);
+    auto load_v = [&](int y0) {
+#pragma unroll
+      for (int y = 0; y < 16; ++y)
+        vw[y] = k_row < 0 || y0 + y >= n ? make_uint2(0, 0) : *reinterpret_cast<const uint2*>(v + (y0 + y) * CHUNK_DIM + (((lane >> 1) ^ (y & 7)) << 3));
+    };
+    load_v(0);
+    float s[16];
+#pragma unroll
+    for (int y = 0; y < 16; ++y) s[y] = dot(q, kw[y]);
+#pragma unroll
+    for (int w = 8; w; w >>= 1)
+#pragma unroll
+      for (int y = 0; y < w; ++y) {
+        const float give = lane & w ? s[y] : s[y + w], keep = lane & w ? s[y + w] : s[y];
+        s[y] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+      }
+    const float d = lane < n ? s[0] * scale : -INFINITY;
+    float top = d;
+#pragma unroll
+    for (int i = 16; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    top = fmaxf(m, top);
+    const float base = top == -INFINITY ? 0.0f : top, f = ex2(m - base), p = ex2(d - base);
+    m = top;
+    l = l * f + p;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[x] *= f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const float2 v01 = TT::to_f32(vw[y].x), v23 = TT::to_f32(vw[y].y);
+        const float py = __shfl_sync(0xffffffffu, p, half * 16 + y), fv[4] = {v01.x, v01.y, v23.x, v23.y};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          o[x] = fmaf(py, fv[x], o[x]);
+          if (want) seen |= kind(fv[x], x);
+        }
+      }
+      if (half == 0) load_v(16);
+    }
+    if (__all_sync(0xffffffffu, (want & ~seen) == 0)) return;
+  }
+#pragma unroll
+  for (int i = 16; i; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+  if (!mine) return;
+  // (a score that is not a number makes l NaN, and m with it for the join)
+  const float f = part ? ex2((l != l ? l : m) - r_m) : 1.0f / l;
+  if (part) *part_at = make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+  else *out_at = make_uint2(TT::from_f32(o[0] * f, o[1] * f), TT::from_f32(o[2] * f, o[3] * f));
 }
 
 // One block's part in a CTA's range, as the walk hands it on.
@@ -854,27 +917,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           mbar_arrive_n(&B.o_free[grp], 2);
         }
       }
-      // rows that came out not finite, one after the other
-      for (unsigned again = __ballot_sync(0xffffffffu, valid && !(bad == 0.0f)); again; again &= again - 1) {
-        const int src = __ffs(again) - 1;
-        const int r_row = __shfl_sync(0xffffffffu, out_row, src), r_head = __shfl_sync(0xffffffffu, qhead, src);
-        const int r_pos = __shfl_sync(0xffffffffu, pos, src), r_prow = __shfl_sync(0xffffffffu, prow, src);
-        const float r_m = __shfl_sync(0xffffffffu, m, src);
-        float rm, rl;
-        float4 o;
-        chunk_row<BF16>(a, d.slot, r_row, r_head, d.t0 * CHUNK_KT, min((d.t0 + nt) * CHUNK_KT, r_pos + 1), rm, rl, o);
-        if (lane >> 3 < c_begin || lane >> 3 >= c_end) continue;  // the other group's dims
-        if (whole) {
-          const float inv = 1.0f / rl;
-          uint2 v;
-          v.x = TT::from_f32(o.x * inv, o.y * inv);
-          v.y = TT::from_f32(o.z * inv, o.w * inv);
-          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(r_row) * a.out_ld + r_head * CHUNK_DIM +
-                                    lane * 4) = v;
-        } else {  // beside the m and l that are there already
-          const float f = ex2(rm - r_m);
-          *reinterpret_cast<float4*>(part + r_prow * CHUNK_PART_LD + lane * 4) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-        }
+      // rows that came out not finite, one after the other (not those with an l that is NaN, a score of their own not being a
+      // number: they are NaN throughout as they should be)
+      for (unsigned again = __ballot_sync(0xffffffffu, valid && l == l && !(bad == 0.0f)); again; again &= again - 1) {
+        const int src = __ffs(again) - 1, r_prow = __shfl_sync(0xffffffffu, prow, src);
+        chunk_row<BF16>(a, d.slot, __shfl_sync(0xffffffffu, out_row, src), __shfl_sync(0xffffffffu, qhead, src), d.t0 * CHUNK_KT,
+                        min((d.t0 + nt) * CHUNK_KT, __shfl_sync(0xffffffffu, pos, src) + 1), lane >> 3 >= c_begin && lane >> 3 < c_end,
+                        whole ? nullptr : part + r_prow * CHUNK_PART_LD, __shfl_sync(0xffffffffu, m, src));
       }
       if (!whole && grp == 0 && row == 0) {
         if (d.t0 == 0) {

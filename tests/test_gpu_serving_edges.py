@@ -172,3 +172,93 @@ def test_chunk_attention_takes_scales_of_any_size(qasr, cuda_device, scale, size
     out = c.run(qasr, scale=scale)
     torch.cuda.synchronize()
     c.check(out, scale=scale)
+
+
+# ------------------------------------------------------------------------------------ values that are not finite
+def _expect_not_finite(c, out, torch):
+    """NaN, infinities and finite outputs where the formula in 64 bits has them: a probability above 0 times an infinite value
+    is infinite, times NaN is NaN, and what a row does not see does not count."""
+    first, G = 0, c.nq // c.nkv
+    for i, (a, b) in enumerate(c.lens):
+        v = c.kv[i][1].float()  # [nkv, positions, dims]
+        seen = [flag.cumsum(1)[:, a:a + b] > 0 for flag in (v.isnan(), v == torch.inf, v == -torch.inf)]
+        nan, plus, minus = (x.permute(1, 0, 2).repeat_interleave(G, 1) for x in seen)  # [rows, nq, dims]
+        nan = nan | (plus & minus)
+        got = out[first:first + b, :c.nq * DIM].view(b, c.nq, DIM)
+        assert torch.equal(got.isnan(), nan), i
+        assert torch.equal(got == torch.inf, plus & ~nan) and torch.equal(got == -torch.inf, minus & ~nan), i
+        first += b
+
+
+def _zeroed(c, torch):
+    """0 for each value that is not finite."""
+    for x in c.kv:
+        x[1] = torch.where(x[1].isfinite(), x[1], torch.zeros_like(x[1]))
+
+
+LENS = [(0, 300), (90, 20), (500, 1), (3000, 1), (2000, 130), (0, 64)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("value", ["nan", "inf", "-inf", "both", "mixed"])
+@pytest.mark.parametrize("where", ["first", "few", "late", "one dim", "all"])
+def test_chunk_attention_of_values_that_are_not_finite(qasr, cuda_device, where, value, dtype):
+    """Prompts, short chunks, whole and cut decode rows, with values that are not finite at the first position, at
+    some, at late ones only (masked for earlier rows of the same block), in one dim, everywhere.  Scores spread so far
+    that f16 probabilities vanish beside the largest; an infinite value still counts there."""
+    import torch
+    c = ops.Chunks(torch, LENS, seed=33, dtype=dtype, spread=2.5)
+    rng = random.Random(7)
+    kinds = {"nan": ["nan"], "inf": ["inf"], "-inf": ["-inf"], "both": ["inf", "-inf"], "mixed": ["nan", "inf", "-inf"]}[value]
+    for kv in c.kv:
+        n = kv.shape[2]
+        at = {"first": [0], "few": [rng.randrange(n) for _ in range(5)], "late": [n - 1 - rng.randrange(min(n, 40)) for _ in range(3)],
+              "one dim": [rng.randrange(n) for _ in range(3)], "all": range(n)}[where]
+        for t in at:
+            dims = slice(0, DIM) if where != "one dim" else rng.randrange(DIM)
+            kv[1, :, t, dims] = float(rng.choice(kinds))
+    c.store()
+    out = c.run(qasr)
+    torch.cuda.synchronize()
+    _expect_not_finite(c, out, torch)
+    # what stays finite, against the formula
+    _zeroed(c, torch)
+    got = out.clone()
+    d = ops.Chunks(torch, LENS, seed=33, dtype=dtype, spread=2.5)
+    d.kv = c.kv
+    d.store()
+    clean = d.run(qasr)
+    torch.cuda.synchronize()
+    d.check(torch.where(got.isfinite(), got, clean))
+
+
+@pytest.mark.parametrize("what,times", [("nan", 30), ("inf", 30), ("one dim", 30), ("late", 200), ("key", 3)])
+def test_one_value_that_is_not_finite_does_not_hold_up_the_call(qasr, cuda_device, what, times):
+    """2048 rows, all of which see it: within 30 times the clean call (about 7 here, 460 when every such row was computed
+    again); when it is masked for most rows of the last block, those are, within 200 times (about 95 here)."""
+    import torch
+    c = ops.Chunks(torch, [(0, 2048)], seed=34)
+    ws = c.workspace(qasr)
+
+    def fastest():
+        best = 1e9
+        for _ in range(5):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            c.run(qasr, ws=ws)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    clean = fastest()
+    x = c.kv[0]
+    if what == "key":
+        x[0, :, 0] = float("nan")
+    elif what == "one dim":
+        x[1, :, 0, 5] = float("nan")
+    else:
+        x[1, :, 2000 if what == "late" else 0] = float("inf" if what == "inf" else "nan")
+    c.store()
+    broken = fastest()
+    assert broken < times * clean
