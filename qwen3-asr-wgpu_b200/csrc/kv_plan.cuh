@@ -9,7 +9,8 @@
 //
 // One cluster does the scans and the pages, and the row maps as well where they are short; long ones (more than
 // PLAN_MAPS_ROWS) are left to kv_row_maps_kernel on all SMs, which expands the finished scan.  (us in a graph, cluster
-// alone / both: 8000 rows 3.7 / 5.1, 16,000 rows 3.9 / 5.2, 1.1 million rows 81 / 9.7.)  Every CTA of the cluster reads the lengths and scans them for itself (a few KB out
+// alone / both: 8000 rows 3.8 / 5.1, 24,000 rows 4.5 / 5.2, 32,000 4.95 / 5.2, 40,000 5.4 / 5.25, 64,000 6.8 / 5.4, 1.1
+// million 81 / 9.8.)  Every CTA of the cluster reads the lengths and scans them for itself (a few KB out
 // of L2, cheaper than handing the sums over); a cluster barrier then stands between the last
 // read and the first write, so that the outputs may be the inputs' own arrays, and the CTAs
 // share the writes.
@@ -22,7 +23,7 @@ namespace qasr {
 
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_MAX_CLUSTER = 8;  // the portable cluster size
-constexpr int PLAN_MAPS_ROWS = 6 * PLAN_MAX_CLUSTER * PLAN_THREADS;
+constexpr int PLAN_MAPS_ROWS = 4 * PLAN_MAX_CLUSTER * PLAN_THREADS;
 
 struct PlanArgs {
   const int* seq_slot;

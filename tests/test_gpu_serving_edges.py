@@ -262,3 +262,20 @@ def test_one_value_that_is_not_finite_does_not_hold_up_the_call(qasr, cuda_devic
     c.store()
     broken = fastest()
     assert broken < times * clean
+
+
+# ------------------------------------------------------------------------------------ plans
+@pytest.mark.parametrize("rows", [32767, 32768, 32769, 49152, 49153])
+@pytest.mark.parametrize("spare", [0, 1])
+def test_kv_plan_where_the_maps_go_to_a_second_kernel(qasr, cuda_device, rows, spare):
+    """The last rows that the planning kernel writes itself and the first that it leaves to the other one, by the room in
+    the maps, which is what is known on the host."""
+    import torch
+    rng = random.Random(rows)
+    new = [rng.randint(0, 1000) for _ in range(60)]
+    new.append(rows - sum(new))
+    assert new[-1] >= 0
+    n, max_pages = len(new), -(-max(new) // PAGE)
+    p = Pages(torch, n, max_pages, n * max_pages, seed=4)
+    slot = rng.sample(range(n), n)
+    ops._check_plan(p, p.plan(qasr, slot, [0] * n, new, rows_cap=rows + spare), slot, [0] * n, new)
