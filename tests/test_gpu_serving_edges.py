@@ -279,3 +279,155 @@ def test_kv_plan_where_the_maps_go_to_a_second_kernel(qasr, cuda_device, rows, s
     p = Pages(torch, n, max_pages, n * max_pages, seed=4)
     slot = rng.sample(range(n), n)
     ops._check_plan(p, p.plan(qasr, slot, [0] * n, new, rows_cap=rows + spare), slot, [0] * n, new)
+
+
+@pytest.mark.parametrize("slot,held,count,want", [
+    ([0, 5], [0, 0], 8, [1, 1]), ([-1, 0], [0, 0], 8, [1, 0]), ([1, 0, 1], [0, 0, 0], 8, [1, 2]), ([1, 0], [257, 0], 8, [1, 0]),
+    ([1, 0], [0, -1], 8, [1, 1]), ([1, 0], [64, 64], -1, [1, -3]), ([1, 0], [64, 64], 21, [1, -3]), ([1, 0], [64, 64], 19, [3, -1]),
+], ids=lambda v: str(v)[:24])
+def test_kv_release_refuses_on_the_device_and_changes_nothing(qasr, cuda_device, slot, held, count, want):
+    import torch
+    p = Pages(torch, 5, 4, 20)
+    p.d_count.fill_(count)
+    s, h, st = _ints(slot, torch), _ints(held, torch), _ints([-9, -9], torch)
+    qasr.kernel_kv_release(0, _stream(torch), s.data_ptr(), h.data_ptr(), len(slot), 5, p.d_table.data_ptr(), 4,
+                           p.d_free.data_ptr(), 20, p.d_count.data_ptr(), h.data_ptr(), p.d_count.data_ptr(), st.data_ptr())
+    torch.cuda.synchronize()
+    assert st.tolist() == want and h.tolist() == held and p.d_count.item() == count
+    assert p.d_free.tolist() == p.free and p.d_table.tolist() == p.table
+
+
+# ------------------------------------------------------------------------------------ outputs written anew
+def test_chunk_attention_on_two_streams_writes_every_row_each_time(qasr, cuda_device):
+    """Two calls at once, each output wiped before each run and compared after it."""
+    import torch
+    c = ops.Chunks(torch, [(700, 90), (1200, 1), (0, 300)] * 3, seed=14)
+    d = ops.Chunks(torch, [(2500, 1)] * 20, seed=15, dtype="bf16")
+    a, b = c.run(qasr).clone(), d.run(qasr).clone()
+    wc, wd = c.workspace(qasr), d.workspace(qasr)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        c.out.fill_(77)
+        d.out.fill_(77)
+        torch.cuda.synchronize()
+        c.run(qasr, ws=wc, stream=s1.cuda_stream)
+        d.run(qasr, ws=wd, stream=s2.cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(a, c.out) and torch.equal(b, d.out)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("which", [0, 1])
+def test_chunk_attention_writes_the_rows_before_a_broken_position(qasr, cuda_device, which, value):
+    import torch
+    c = ops.Chunks(torch, [(90, 200), (0, 40), (300, 1)], seed=10)
+    kv = [x.clone() for x in c.kv]
+    c.kv[0][which, :, 90 + 150] = value
+    c.kv[1][which, :, 39] = value
+    c.store()
+    out = c.run(qasr)  # into an output that no run has written
+    torch.cuda.synchronize()
+    c.kv = kv
+    c.check(out, skip=set(range(150, 200)) | {239})
+
+
+def test_calls_for_another_device_leave_the_current_one_alone(qasr, cuda_device):
+    import torch
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    w = ops.W4(qasr, torch, 64, 64, 64, False, "f16", 1)
+    c = ops.Chunks(torch, [(0, 4)])
+    stream = torch.cuda.current_stream(0).cuda_stream
+    torch.cuda.synchronize()
+    with torch.cuda.device(1):
+        qasr.kernel_gemv_w4(0, stream, qasr.TYPE_F16, w.packed.data_ptr(), False, 64, 64, 64, w.x.data_ptr(), 64, 1,
+                            w.out.data_ptr(), 64)
+        c.run(qasr, stream=stream)
+        assert torch.cuda.current_device() == 1
+    torch.cuda.synchronize()
+    w.check(w.out)
+    c.check(c.out)
+
+
+# ------------------------------------------------------------------------------------ a step of all operators, bf16, room to spare
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_a_captured_serving_step_with_room_for_more_rows(qasr, cuda_device, dtype):
+    """Plan, 4-bit q|k|v product, planned append, attention, 4-bit output product in one graph with room for 64 rows,
+    replayed with chunks, single tokens, an idle request and a step that is refused in between."""
+    import torch
+    t = torch.bfloat16 if dtype == "bf16" else torch.float16
+    hs, nq, nkv, max_pages, slots, pool_pages, cap, n = 512, 16, 8, 4, 6, 14, 64, 3
+    p = Pages(torch, slots, max_pages, pool_pages, seed=8)
+    pool = torch.full((pool_pages, 1, 2, nkv, PAGE, DIM), float("nan"), dtype=t, device="cuda")
+    qkv = ops.W4(qasr, torch, (nq + 2 * nkv) * DIM, hs, 64, True, dtype, cap, seed=1)
+    o = ops.W4(qasr, torch, hs, nq * DIM, 128, False, dtype, cap, seed=2)
+    qkv.scale.mul_(0.3)
+    qasr.kernel_pack_w4(0, _stream(torch), qkv.codes.data_ptr(), qkv.scale.data_ptr(), qkv.zero.data_ptr(), qkv.n_out, hs, 64,
+                        qkv.packed.data_ptr())
+    ws_bytes = qasr.kernel_attention_chunk_workspace(0)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
+    slot, held = [4, 0, 3], [0, 0, 0]
+    d_slot, d_len, d_new = _ints(slot, torch), _ints(held, torch), _ints([0] * n, torch)
+    cu, status = _ints([0] * (n + 1), torch), _ints([0, 0], torch)
+    maps = [_ints([2**31 - 1] * cap, torch) for _ in range(2)]
+    k, v = (torch.empty((cap, nkv * DIM), dtype=t, device="cuda") for _ in range(2))
+    att = torch.empty((cap + 1, nq * DIM), dtype=t, device="cuda")
+    y = qkv.out
+    o.x = att
+
+    def step():
+        st = _stream(torch)
+        qasr.kernel_kv_plan(0, st, d_slot.data_ptr(), d_len.data_ptr(), d_new.data_ptr(), n, slots, p.d_table.data_ptr(), max_pages,
+                            p.d_free.data_ptr(), pool_pages, p.d_count.data_ptr(), d_len.data_ptr(), p.d_count.data_ptr(),
+                            cu.data_ptr(), maps[0].data_ptr(), maps[1].data_ptr(), cap, status.data_ptr())
+        qkv.run(qasr)
+        k.copy_(y[:cap, nq * DIM:(nq + nkv) * DIM])
+        v.copy_(y[:cap, (nq + nkv) * DIM:])
+        qasr.kernel_kv_append_planned(0, st, k.data_ptr(), v.data_ptr(), pool.data_ptr(), pool_pages, p.d_table.data_ptr(), slots,
+                                      max_pages, 1, nkv, 0, maps[0].data_ptr(), maps[1].data_ptr(), cap, cu.data_ptr() + 4 * n)
+        qasr.kernel_attention_chunk(0, st, qasr.TYPE_BF16 if dtype == "bf16" else qasr.TYPE_F16, y.data_ptr(), y.shape[1],
+                                    att.data_ptr(), nq * DIM, cap, pool.data_ptr(), pool_pages, p.d_table.data_ptr(), slots,
+                                    max_pages, 1, nq, nkv, 0, d_slot.data_ptr(), cu.data_ptr(), d_len.data_ptr(), n, ws.data_ptr(),
+                                    ws_bytes)
+        o.run(qasr, accumulate=True)
+
+    step()  # a step of no rows: also the first call of each, ahead of the capture
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    cache = {s: torch.empty((2, nkv, 0, DIM), dtype=t, device="cuda") for s in slot}
+    for new, refused in [([30, 21, 13], 0), ([1, 1, 1], 0), ([40, 40, 1], 1), ([20, 0, 40], 0), ([1, 300, 1], 1), ([1, 1, 1], 0)]:
+        d_new.copy_(_ints(new, torch))
+        qkv.x.copy_(torch.randn_like(qkv.x))
+        att.fill_(77)
+        o.out[:cap] = torch.randn((cap, hs), device="cuda").to(t)
+        resid, before = o.out[:cap].clone(), pool.clone()
+        graph.replay()
+        qasr.kernel_attention_chunk_check(0, _stream(torch), ws.data_ptr())
+        qasr.kernel_gemv_w4_check(0, _stream(torch))
+        torch.cuda.synchronize()
+        qkv.check(y)
+        if refused:
+            assert status.tolist()[0] == 3 and d_len.tolist() == held
+            assert torch.equal(pool.view(torch.int16), before.view(torch.int16)) and (att == 77).all()
+            continue
+        rows = sum(new)
+        p.expect(slot, held, new)
+        assert status.tolist() == [0, 0] and p.d_table.tolist() == p.table
+        c = ops.Chunks.__new__(ops.Chunks)
+        c.torch, c.t, c.nq, c.nkv, c.rows, c.lens = torch, t, nq, nkv, rows, list(zip(held, new))
+        c.q, c.kv, first = y[:, :nq * DIM], [], 0
+        for i, s in enumerate(slot):
+            add = torch.stack([k[first:first + new[i]], v[first:first + new[i]]]).view(2, new[i], nkv, DIM).transpose(1, 2)
+            cache[s] = torch.cat([cache[s], add], 2)
+            c.kv.append(cache[s])
+            first += new[i]
+        c.check(att)
+        held = [a + b for a, b in zip(held, new)]
+        assert d_len.tolist() == held
+        o.x = att[:cap]
+        o.check(o.out, before=resid)
+        o.x = att
