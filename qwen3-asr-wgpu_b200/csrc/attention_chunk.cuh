@@ -34,11 +34,13 @@
 // partials (o, m, l) in the workspace and attention_chunk_combine_kernel joins them, in key order.
 // Nothing about the lengths is known on the host: every CTA sums the costs itself.
 //
-// Measured (B200, us in a graph): 512 slots of 256-4096 positions 690-735 (6.1-6.5 TB/s, 94-99% of the measured copy rate),
-// 32 slots of 100-1500 31, one token over 224 positions 10.6 (latency: launch 2, first block found 3, pages 1, three
-// dependent products and softmaxes 3, join 2), 64 requests of 13 rows 62-74, 8192 rows from nothing 247 (1110
-// TFLOP/s, 68% of measured bf16): the chain P -> P V -> Q K^T -> S of each group takes about 1850 cycles for 64 keys where the
-// tensor cores need 1280 for both groups' products and the exponential unit 768.
+// Measured (B200, us a call in a graph; first a burst of milliseconds, then under the power cap after seconds of nothing
+// else, with the SM clock seen): 512 slots of 256-4096 positions 712 (6.3 TB/s, 96% of the measured copy rate) / 845 (1450 MHz), 8192
+// rows from nothing 252 (1090 TFLOP/s, 66% of measured bf16) / 294 (1545 MHz; 935 TFLOP/s, 67% of the sustained rate).  Bursts:
+// 32 slots of 100-1500 31, one token over 224 positions 10.8 (latency: launch 2, first block found 3, pages 1, three
+// dependent products and softmaxes 3, join 2), 64 requests of 13 rows 58-76.  With 8192 rows the chain P -> P V -> Q K^T -> S of
+// each group takes about 1850 cycles for 64 keys where the tensor cores need 1280 for both groups' products and the exponential unit
+// 768: what is long is S to P, 1300 cycles of one thread's row in which no unit is busy half of the time.
 //
 // Masked keys: S is replaced, never added to, so whatever stands there cannot matter; their P is 0, and
 // V rows behind the block's last position are zeroed in shared memory, so that 0 * NaN cannot arise.  What remains
@@ -84,7 +86,7 @@ constexpr int CHUNK_Q_TILE = 128 * CHUNK_DIM * 2, CHUNK_Q_HALF = CHUNK_Q_TILE / 
 constexpr int CHUNK_Q_BYTES = 2 * CHUNK_Q_TILE;
 constexpr int CHUNK_OUT_BYTES = 32 * 64;           // per softmax warp: a quarter of its rows' output
 constexpr int CHUNK_SMEM = CHUNK_Q_BYTES + (CHUNK_K_STAGES + CHUNK_V_STAGES) * CHUNK_STAGE_BYTES + 8 * CHUNK_OUT_BYTES + 3 * 1024;  // (m and l, ChunkBars)
-constexpr int CHUNK_BLOCK_COST = 4;               // a block's Q copy, first and last steps, in key tiles (2: 32 slots 33.7 us, 4: 30.9, 6: 31.6)
+constexpr int CHUNK_BLOCK_COST = 4;               // a block's Q copy, first and last steps, in key tiles (us at 2 / 4 / 6: 32 slots 34.1 / 31.3 / 31.3, 512 slots 700 / 683 / 684, 64 x 13 rows 70-82 / 58-63 / 62-69, a mixed step 71-75 / 68-71 / 72-74)
 constexpr int CHUNK_SNAP = 2;                     // a cut this near to a block's edge moves onto it
 constexpr float CHUNK_RESCALE = 8.0f;
 constexpr uint32_t CHUNK_WAIT_STEPS = (10 * QASR_WAIT_NS) >> 20;  // chunk_row keeps the others waiting: 2.6 s for 32 rows of 2^20 positions
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             // every fourth pair on the FMA pipe, so that the exponential unit is not what a tile waits for (8192 rows: none
-            // 261 us, a fourth 247, a third 250)
+            // 261 us, a fourth 247, a third 250 at the time; 252 now)
             const uint64_t e = fma2(pack2(s[2 * c], s[2 * c + 1]), scale2, base2);
             float p0, p1;
             if (c % 4 == 3) {
@@ -829,7 +831,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           return v;
         };
         float* my_part = part + prow * CHUNK_PART_LD;
-        if (__popc(rows_valid) <= 4) {  // as in a decode step: straight out of the rows' threads (32 slots: 31.1 us, through shared memory 32.2)
+        if (__popc(rows_valid) <= 4) {  // as in a decode step: straight out of the rows' threads (us, through shared memory / straight: 32 slots of two rows 32.2 / 31.3, one token 11.1 / 10.8; of eight rows 21-23 / 22-24)
           T* to = static_cast<T*>(a.out) + static_cast<size_t>(out_row) * a.out_ld + qhead * CHUNK_DIM;
 #pragma unroll 1
           for (int c = c_begin; c < c_end; ++c) {

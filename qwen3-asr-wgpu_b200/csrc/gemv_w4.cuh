@@ -166,10 +166,11 @@ struct W4Type<true> {
 // order.  x comes through L1, where it stays.  When there are few row tiles, the CTAs of a cluster share their k as well
 // and the first joins their sums, in order.
 // NT = ceil(rows / 8): the rows of x are the matrix instruction's eight columns, NT times over.  A weight is read and
-// taken apart once whatever the rows are; at 8 rows and below this taking apart (9 instructions per 8 weights and lane)
-// is what comes closest to the memory's pace.  Measured (B200, us in a graph): 151936 x 2048 at one row 34.5 (4.7 TB/s), 60000
-// x 8192 at one row 49.9 (5.1 TB/s, 78% of the measured copy rate), at 16 rows 76, at 32 rows 150 (there x's way from
-// L1 and the matrix instructions bound it), 2048 x 6144 at one row 4.4, 1024 x 2048 2.7 (latency).
+// taken apart once whatever the rows are (9 instructions per 8 weights and lane).  Measured (B200, us in a graph): 60000 x 8192 at one
+// row 50 (5.1 TB/s, 78% of the measured copy rate), 8 rows 55, 16 rows 76, 32 rows 148 (there x's way from L1 and the matrix
+// instructions bound it), 33 rows 260 and 64 rows 280 (255 registers a thread and spills), 151936 x 2048 at one row 35 (4.6
+// TB/s, 37.5 under the power cap: a warp has only two units between the joins of its tile), 2048 x 6144 at one row 4.4,
+// 1024 x 2048 2.8 (latency).
 // A wait for a copy that gives up is recorded in w4_status, and every output whose sum then lacks a part is NaN.
 constexpr int W4_WARPS = 8;
 constexpr int W4_THREADS = W4_WARPS * 32;
